@@ -2,8 +2,8 @@
  * mfb.h — C ABI of the B200 (sm_100a) dense FP32 contraction library (libmfb.so).
  *
  * Every entry point takes plain pointers, sizes and a CUDA stream handle; no C++
- * or framework types cross this boundary. All matrices are row-major FP32 with
- * explicit leading dimensions (elements), exactly like the reference's pointer
+ * or framework types cross this boundary. All matrices are row-major (FP32 where no
+ * mfb_dtype_t says otherwise) with explicit leading dimensions (elements), exactly like the reference's pointer
  * interface. Buffers are caller-owned device memory unless stated otherwise.
  *
  * Replaces (reference file:line):
@@ -35,6 +35,9 @@
  *                                   (src/nn/conv.cu:110-163)
  *   mfb_naive_sgemm                 the one-thread-per-output comparison GEMM
  *                                   benchmarks/bench_comparison.cu:76 (device correctness oracle)
+ * Without a counterpart in the reference: mfb_grouped_gemm / _bwd_right (products grouped by
+ * expert) and mfb_quantize_int4 / _dequantize_int4 / mfb_gemv_int4 (4-bit weights), which also
+ * take 16-bit operands (mfb_dtype_t).
  */
 #ifndef MFB_H_
 #define MFB_H_
@@ -102,14 +105,15 @@ MFB_API const char* mfb_last_error(void);
 MFB_API const char* mfb_version(void);
 
 /* Reads and clears the device status word that bounded waits report into.
- * *bits receives the raw word (0 = no timeout since the last read). Synchronizes
- * the device first. Returns MFB_ETIMEOUT when any bit was set. */
+ * *bits receives the raw word (0 = nothing reported since the last read). Synchronizes
+ * the device first. Returns MFB_ETIMEOUT when a wait gave up, MFB_EINVAL when kernels only
+ * found group offsets or expert ids out of range. */
 MFB_API mfb_status_t mfb_device_status(int device, uint32_t* bits);
 /* Bound, in nanoseconds of device time, for every device-side wait of later launches
  * (default 4e9 = 4 s). Process-wide. */
 MFB_API mfb_status_t mfb_set_wait_limit_ns(uint64_t limit_ns);
 MFB_API uint64_t mfb_get_wait_limit_ns(void);
-/* Synchronizes `stream` on `device`, then reports CUDA errors and device timeouts. */
+/* Synchronizes `stream` on `device`, then reports CUDA errors and the device status word. */
 MFB_API mfb_status_t mfb_sync(int device, mfb_stream_t stream);
 
 /* ---------------------------------------------------------------- hw::cuda_gemm drop-in */
@@ -311,6 +315,74 @@ MFB_API mfb_status_t mfb_covariance(int device, mfb_stream_t stream, int rows, i
                                     float* cov, int ldcov, int precision);
 MFB_API mfb_status_t mfb_correlation(int device, mfb_stream_t stream, int rows, int cols, const float* x, int ldx,
                                      float* corr, int ldcorr, int precision);
+
+/* ---------------------------------------------------------------- products grouped by expert */
+/* Element types of the grouped products and the 4-bit matrices. */
+typedef enum mfb_dtype_t { MFB_DTYPE_F32 = 0, MFB_DTYPE_F16 = 1, MFB_DTYPE_BF16 = 2 } mfb_dtype_t;
+
+/* Groups of consecutive rows with a matrix each: the experts of a mixture-of-experts layer.
+ * offsets (device memory, groups + 1 ints, not decreasing): group e holds rows
+ * [offsets[e], offsets[e + 1]), which may be none. They are read by the kernels, so the host
+ * needs no group size and a captured graph follows new offsets on replay. Offsets below 0,
+ * above `rows` or smaller than an earlier one are clamped (nothing out of bounds is touched)
+ * and reported as MFB_EINVAL by the next mfb_sync / mfb_device_status. groups <= 4096. */
+typedef struct mfb_grouped_desc {
+    int groups; /* experts */
+    int rows;   /* rows of A (and of C, or of B in mfb_grouped_gemm_bwd_right) */
+    int n, k;
+    int lda, ldb, ldc;  /* row strides in elements */
+    long long stride;   /* elements between the groups' matrices: B of mfb_grouped_gemm (0: all groups
+                         * share one), C of mfb_grouped_gemm_bwd_right */
+    int dtype;          /* mfb_dtype_t of A and B */
+    int out_dtype;      /* dtype or MFB_DTYPE_F32 */
+    int precision;      /* mfb_precision_t, for MFB_DTYPE_F32 operands */
+    int trans_b;        /* mfb_grouped_gemm: B is stored n x k */
+    int zero_rest;      /* mfb_grouped_gemm: rows outside every group become 0; else they stay as they were */
+} mfb_grouped_desc;
+
+/* C[t] = A[t] * op(B_e) for every row t of group e: A rows x k, B_e k x n (n x k with trans_b),
+ * C rows x n. Products of the operands' own bits, sums in FP32, one rounding to out_dtype; FP32
+ * operands as three BF16 terms each (strict) or two (MFB_PRECISION_TF32). The gradient by A is
+ * the same call on the gradient rows with trans_b flipped. k == 0 gives 0. Takes no scratch. */
+MFB_API mfb_status_t mfb_grouped_gemm(int device, mfb_stream_t stream, const mfb_grouped_desc* desc,
+                                      const int* offsets, const void* a, const void* b, void* c);
+/* C_e = sum over rows t of group e of A[t]^T B[t] (k x n; A rows x k, B rows x n): the gradient by
+ * the groups' matrices. A group without rows gives 0. trans_b and zero_rest must be 0 (swap A and
+ * B for the transposed result). Takes no scratch; sums in a fixed order. */
+MFB_API mfb_status_t mfb_grouped_gemm_bwd_right(int device, mfb_stream_t stream, const mfb_grouped_desc* desc,
+                                                const int* offsets, const void* a, const void* b, void* c);
+
+/* ---------------------------------------------------------------- 4-bit weights */
+/* n x k weights (or a stack of `experts` of them) as 4-bit codes q with one scale s (and zero point
+ * z, 8 where `zeros` is NULL) per row and group of `group` consecutive columns: w = (q - z) * s.
+ * Column j of a row is in byte j / 2, even j in the low half; rows take 16 * ceil(k / 32) bytes
+ * (what is behind column k is ignored); scales and zeros are n x ceil(k / group), all contiguous. */
+typedef struct mfb_int4_matrix {
+    unsigned char* packed;  /* 16-byte aligned */
+    void* scales;           /* scale_dtype */
+    unsigned char* zeros;   /* 0..15 each, or NULL */
+    int experts;            /* matrices in the stack (>= 1) */
+    int n, k;
+    int group;              /* 32, 64 or 128 */
+    int scale_dtype;        /* mfb_dtype_t */
+} mfb_int4_matrix;
+
+/* Codes of w (element strides: row ldw, matrix stride_w; finite values). With zeros: over a group,
+ * lo = min(0, w), hi = max(0, w), s = (hi - lo) / 15, z = rint(-lo / s); without: s = max|w| / 7.
+ * s is rounded to scale_dtype (saturating; 0 becomes 1) before the codes, q = rint(w / s) + z
+ * clamped to 0..15, ties to even, decided on the exact quotient. */
+MFB_API mfb_status_t mfb_quantize_int4(int device, mfb_stream_t stream, const void* w, int dtype, long long ldw,
+                                       long long stride_w, const mfb_int4_matrix* out);
+/* out = (q - z) * s, rounded once to `dtype`. */
+MFB_API mfb_status_t mfb_dequantize_int4(int device, mfb_stream_t stream, const mfb_int4_matrix* m, void* out,
+                                         int dtype, long long ldo, long long stride_o);
+/* y[r] = W x[r] for rows r of x (rows x k, row stride ldx) and y (rows x n, row stride ldy), both of
+ * `dtype`; the products take the codes exactly and sums are FP32. rows <= MFB_INT4_GEMV_ROWS. With
+ * expert_ids (device memory, one int per row) row r uses matrix expert_ids[r] of the stack; a negative
+ * id gives a zero row, one >= experts a zero row and MFB_EINVAL from the next mfb_sync. */
+#define MFB_INT4_GEMV_ROWS 64
+MFB_API mfb_status_t mfb_gemv_int4(int device, mfb_stream_t stream, const mfb_int4_matrix* m, int rows, const void* x,
+                                   long long ldx, int dtype, const int* expert_ids, void* y, long long ldy);
 
 /* ---------------------------------------------------------------- GEMV / skinny */
 /* Bandwidth-bound FP32 kernel for n <= 16 (y = A x with ldb/ldc strides) and for

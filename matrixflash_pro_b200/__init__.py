@@ -3,7 +3,8 @@
 Drop-in for MatrixFlash-Pro's GEMM / GEMV / conv2d-forward hot path:
 ``cuda_gemm``/``cuda_sync`` (hw layer), ``GemmPlan``/``gemm``/``gemm_into``
 (Matrix API), ``gemv``, ``conv2d`` forward and backward, the strided-batched ``batch_matmul`` family and
-``covariance``/``correlation``.
+``covariance``/``correlation``. For mixture-of-experts layers: ``grouped_matmul`` and its gradients (rows grouped by
+expert) and 4-bit weights (``quantize_int4``, ``dequantize_int4``, ``gemv_int4``).
 All arithmetic runs in libmfb.so
 (hand-written tcgen05/TMA kernels); there is no CPU fallback.
 """
@@ -18,6 +19,8 @@ from .conv import (conv2d, conv2d_bias_backward, conv2d_input_backward, conv2d_i
                    conv2d_weight_backward)
 from .batch import (batch_matmul, batch_matmul_backward_left, batch_matmul_backward_right,  # noqa: F401
                     sgemm_strided_batched)
+from .grouped import grouped_matmul, grouped_matmul_backward_left, grouped_matmul_backward_right  # noqa: F401
+from .int4 import Int4Matrix, dequantize_int4, gemv_int4, quantize_int4  # noqa: F401
 from .stats import correlation, covariance  # noqa: F401
 from . import collectives  # noqa: F401
 from ._lib import LIB_PATH, lib  # noqa: F401

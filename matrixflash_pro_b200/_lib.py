@@ -26,7 +26,8 @@ EXPORTED_SYMBOLS = (
     "mfb_conv2d_fwd", "mfb_naive_sgemm", "mfb_probe_wait_timeout", "mfb_covariance", "mfb_correlation",
     "mfb_probe_tf32_mma_tflops", "mfb_conv2d_bwd_data", "mfb_conv2d_bwd_filter", "mfb_conv2d_bwd_bias",
     "mfb_all_reduce", "mfb_broadcast", "mfb_all_gather", "mfb_reduce_scatter", "mfb_scatter", "mfb_gather",
-    "mfb_cuda_nccl_allreduce",
+    "mfb_cuda_nccl_allreduce", "mfb_grouped_gemm", "mfb_grouped_gemm_bwd_right", "mfb_quantize_int4",
+    "mfb_dequantize_int4", "mfb_gemv_int4",
 )
 
 
@@ -46,6 +47,21 @@ class CollectiveBuffer(ctypes.Structure):
 class RowBlock(ctypes.Structure):
     """mfb_row_block (include/mfb.h)."""
     _fields_ = [("device", ctypes.c_int), ("rows", ctypes.c_int), ("a", ctypes.c_void_p), ("c", ctypes.c_void_p)]
+
+
+class GroupedDesc(ctypes.Structure):
+    """mfb_grouped_desc (include/mfb.h)."""
+    _fields_ = [("groups", ctypes.c_int), ("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int),
+                ("lda", ctypes.c_int), ("ldb", ctypes.c_int), ("ldc", ctypes.c_int), ("stride", ctypes.c_longlong),
+                ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("precision", ctypes.c_int),
+                ("trans_b", ctypes.c_int), ("zero_rest", ctypes.c_int)]
+
+
+class Int4MatrixDesc(ctypes.Structure):
+    """mfb_int4_matrix (include/mfb.h)."""
+    _fields_ = [("packed", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
+                ("experts", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("group", ctypes.c_int),
+                ("scale_dtype", ctypes.c_int)]
 
 
 class PlanInfo(ctypes.Structure):
@@ -117,6 +133,14 @@ def _declare(lib):
         "mfb_conv2d_fwd": (st, [ctypes.c_int, _vp] + [ctypes.c_int] * 9 + [_vp, _vp, _vp, _vp, ctypes.c_int]),
         "mfb_naive_sgemm": (st, [ctypes.c_int, _vp, ctypes.POINTER(GemmDesc), _vp, _vp, _vp, _vp]),
         "mfb_probe_wait_timeout": (st, [ctypes.c_int, _vp, ctypes.c_uint64]),
+        "mfb_grouped_gemm": (st, [ctypes.c_int, _vp, ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp]),
+        "mfb_grouped_gemm_bwd_right": (st, [ctypes.c_int, _vp, ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp]),
+        "mfb_quantize_int4": (st, [ctypes.c_int, _vp, _vp, ctypes.c_int, ctypes.c_longlong, ctypes.c_longlong,
+                                   ctypes.POINTER(Int4MatrixDesc)]),
+        "mfb_dequantize_int4": (st, [ctypes.c_int, _vp, ctypes.POINTER(Int4MatrixDesc), _vp, ctypes.c_int,
+                                     ctypes.c_longlong, ctypes.c_longlong]),
+        "mfb_gemv_int4": (st, [ctypes.c_int, _vp, ctypes.POINTER(Int4MatrixDesc), ctypes.c_int, _vp,
+                               ctypes.c_longlong, ctypes.c_int, _vp, _vp, ctypes.c_longlong]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

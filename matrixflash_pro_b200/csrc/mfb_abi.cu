@@ -167,6 +167,8 @@ mfb_status_t read_and_clear_status(uint32_t* bits) {
     const uint32_t zero = 0;
     MFB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)), "status clear");
     if (bits) *bits = v;
+    if (v == kStatusBadIndex)
+        return fail(MFB_EINVAL, "a kernel found group offsets or an expert id out of range");
     return v ? fail(MFB_ETIMEOUT, "a bounded device wait gave up (status 0x" + std::to_string(v) + ")") : MFB_OK;
 }
 

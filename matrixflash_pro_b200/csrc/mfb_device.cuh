@@ -8,15 +8,17 @@
 
 namespace mfb {
 
-// Status bits a kernel ORs into g_status when it gives up on a wait. The host
-// reads and clears the word (mfb_sync / mfb_device_status) and maps any set bit
-// to MFB_ETIMEOUT.
+// Status bits a kernel ORs into g_status when it gives up on a wait or finds an index in
+// device memory out of range. The host reads and clears the word (mfb_sync /
+// mfb_device_status) and maps kStatusBadIndex alone to MFB_EINVAL, any other bit to
+// MFB_ETIMEOUT.
 enum : uint32_t {
     kStatusTimeoutProducer = 1u << 0,   // TMA producer waited too long for a free stage
     kStatusTimeoutMma = 1u << 1,        // MMA issuer waited too long for a filled stage
     kStatusTimeoutEpilogue = 1u << 2,   // epilogue waited too long for the accumulator
     kStatusTimeoutDrain = 1u << 3,      // teardown waited too long for in-flight copies/MMAs
     kStatusTimeoutProbe = 1u << 4,      // the bounded-wait probe kernel (mfb_probe_wait_timeout)
+    kStatusBadIndex = 1u << 5,          // group offsets or an expert id out of range
     kStatusBadLaunch = 1u << 8,         // kernel saw launch parameters it cannot serve
 };
 

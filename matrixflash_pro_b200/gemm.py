@@ -116,7 +116,8 @@ def sgemm_ptr(device: int, stream: int, desc, a: int, b: int, c: int, bias: int 
 
 
 def sync(device: int | None = None, stream=None) -> None:
-    """Synchronize a stream and surface device-side timeouts as DeviceTimeoutError."""
+    """Synchronize a stream and surface device-side timeouts as DeviceTimeoutError, indices that a
+    kernel found out of range as InvalidArgumentError."""
     dev = torch.cuda.current_device() if device is None else device
     _lib.check(_lib.lib().mfb_sync(dev, _stream_handle(stream)), "sync")
 
@@ -131,11 +132,12 @@ def probe_tf32_mma_tflops(n: int = 256, device: int | None = None) -> float:
 
 
 def device_status(device: int | None = None) -> int:
-    """Read and clear the device status word (0 = no bounded wait gave up)."""
+    """Read and clear the device status word (0 = no bounded wait gave up and no kernel found
+    an index out of range)."""
     dev = torch.cuda.current_device() if device is None else device
     bits = ctypes.c_uint32(0)
     st = _lib.lib().mfb_device_status(dev, ctypes.byref(bits))
-    if st not in (_lib.MFB_OK, _lib.MFB_ETIMEOUT):
+    if st not in (_lib.MFB_OK, _lib.MFB_ETIMEOUT) and not bits.value:
         _lib.check(st, "device_status")
     return int(bits.value)
 
