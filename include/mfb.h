@@ -325,7 +325,7 @@ typedef enum mfb_dtype_t { MFB_DTYPE_F32 = 0, MFB_DTYPE_F16 = 1, MFB_DTYPE_BF16 
  * [offsets[e], offsets[e + 1]), which may be none. They are read by the kernels, so the host
  * needs no group size and a captured graph follows new offsets on replay. Offsets below 0,
  * above `rows` or smaller than an earlier one are clamped (nothing out of bounds is touched)
- * and reported as MFB_EINVAL by the next mfb_sync / mfb_device_status. groups <= 4096. */
+ * and reported as MFB_EINVAL by the next mfb_sync / mfb_device_status. groups <= 1024. */
 typedef struct mfb_grouped_desc {
     int groups; /* experts */
     int rows;   /* rows of A (and of C, or of B in mfb_grouped_gemm_bwd_right) */

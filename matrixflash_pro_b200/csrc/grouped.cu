@@ -1,171 +1,15 @@
 // Products grouped by expert: C[t] = A[t] op(B_e) for the rows t of group e, and the gradient by the
 // groups' matrices C_e = sum_t A[t]^T B[t]. Group sizes are device data (row offsets), read by the
 // kernels, so nothing here waits for the host.
+#include "grouped_tc.cuh"
 #include "mfb_internal.h"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include <algorithm>
+#include <map>
+#include <mutex>
 
 namespace mfb {
 namespace {
-
-constexpr int kMaxGroups = 4096;
-
-struct GroupedParams {
-    const int* offsets;
-    int groups, rows, n, k;
-    long long lda, ldb, ldc, stride;
-    int trans_b, zero_rest;
-    const void* a;
-    const void* b;
-    void* c;
-};
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) {
-    return v;
-}
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) {
-    return __float2half_rn(v);
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
-    return __float2bfloat16_rn(v);
-}
-
-// Offset e, clamped to [previous, rows]; anything else is reported.
-__device__ __forceinline__ int checked_offset(const GroupedParams& p, int e, int previous) {
-    const int v = p.offsets[e];
-    const int c = min(max(v, previous), p.rows);
-    if (c != v) atomicOr(&g_status, kStatusBadIndex);
-    return c;
-}
-
-// 64 x 64 tiles of C, 16 x 16 threads of 4 x 4 sums. blockIdx.y counts the 64-row tiles of the groups in
-// turn (each group starts a tile of its own, so at most ceil(rows / 64) + groups are used).
-template <typename T, typename TO>
-__global__ void __launch_bounds__(256) grouped_simple_kernel(const GroupedParams p) {
-    __shared__ float as[16][65], bs[16][65];
-    __shared__ int s_e, s_t0, s_t1;
-    if (threadIdx.x == 0) {
-        int tile = blockIdx.y, start = checked_offset(p, 0, 0);
-        s_e = -1;
-        for (int e = 0; e < p.groups; ++e) {
-            const int end = checked_offset(p, e + 1, start);
-            const int tiles = (end - start + 63) / 64;
-            if (tile < tiles) {
-                s_e = e;
-                s_t0 = start + tile * 64;
-                s_t1 = min(end, s_t0 + 64);
-                break;
-            }
-            tile -= tiles;
-            start = end;
-        }
-    }
-    __syncthreads();
-    if (s_e < 0) return;
-    const int t0 = s_t0, t1 = s_t1, j0 = blockIdx.x * 64;
-    const T* a = static_cast<const T*>(p.a);
-    const T* b = static_cast<const T*>(p.b) + p.stride * s_e;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float sum[4][4] = {}, part[4][4] = {};  // a chain of 64 products at a time, then the chains' sum
-    for (int k0 = 0; k0 < p.k; k0 += 16) {
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int r = i / 16, c = i % 16;
-            as[c][r] = t0 + r < t1 && k0 + c < p.k ? to_f32(a[(t0 + r) * p.lda + k0 + c]) : 0.0f;
-            const int kk = p.trans_b ? i % 16 : i / 64, jj = p.trans_b ? i / 16 : i % 64;
-            const bool in = j0 + jj < p.n && k0 + kk < p.k;
-            const long long at = p.trans_b ? (j0 + jj) * p.ldb + k0 + kk : (k0 + kk) * p.ldb + j0 + jj;
-            bs[kk][jj] = in ? to_f32(b[at]) : 0.0f;
-        }
-        __syncthreads();
-        for (int kk = 0; kk < 16; ++kk)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) part[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx * 4 + j], part[i][j]);
-        if ((k0 / 16) % 4 == 3 || k0 + 16 >= p.k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) {
-                    sum[i][j] += part[i][j];
-                    part[i][j] = 0.0f;
-                }
-        __syncthreads();
-    }
-    TO* c = static_cast<TO*>(p.c);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int t = t0 + ty * 4 + i, col = j0 + tx * 4 + j;
-            if (t < t1 && col < p.n) c[t * p.ldc + col] = from_f32<TO>(sum[i][j]);
-        }
-}
-
-// C_e (k x n) = sum over the group's rows of A[t]^T B[t]; blockIdx.z = group.
-template <typename T, typename TO>
-__global__ void __launch_bounds__(256) grouped_right_simple_kernel(const GroupedParams p) {
-    __shared__ float as[16][65], bs[16][65];
-    __shared__ int s_t0, s_t1;
-    if (threadIdx.x == 0) {
-        int start = checked_offset(p, 0, 0), end = start;
-        for (int e = 0; e <= static_cast<int>(blockIdx.z); ++e) {
-            start = end;
-            end = checked_offset(p, e + 1, start);
-        }
-        s_t0 = start;
-        s_t1 = end;
-    }
-    __syncthreads();
-    const int t0 = s_t0, t1 = s_t1, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-    const T* a = static_cast<const T*>(p.a);
-    const T* b = static_cast<const T*>(p.b);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float sum[4][4] = {}, part[4][4] = {};
-    for (int t = t0; t < t1; t += 16) {
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int r = i / 64, c = i % 64;
-            as[r][c] = t + r < t1 && i0 + c < p.k ? to_f32(a[(t + r) * p.lda + i0 + c]) : 0.0f;
-            bs[r][c] = t + r < t1 && j0 + c < p.n ? to_f32(b[(t + r) * p.ldb + j0 + c]) : 0.0f;
-        }
-        __syncthreads();
-        for (int kk = 0; kk < 16; ++kk)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) part[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx * 4 + j], part[i][j]);
-        if (((t - t0) / 16) % 4 == 3 || t + 16 >= t1)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) {
-                    sum[i][j] += part[i][j];
-                    part[i][j] = 0.0f;
-                }
-        __syncthreads();
-    }
-    TO* c = static_cast<TO*>(p.c) + p.stride * blockIdx.z;
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int row = i0 + ty * 4 + i, col = j0 + tx * 4 + j;
-            if (row < p.k && col < p.n) c[row * p.ldc + col] = from_f32<TO>(sum[i][j]);
-        }
-}
-
-// Zeros in the rows that belong to no group.
-template <typename TO>
-__global__ void __launch_bounds__(256) grouped_rest_kernel(const GroupedParams p) {
-    __shared__ int s_first, s_last;
-    if (threadIdx.x == 0) {
-        int last = s_first = checked_offset(p, 0, 0);
-        for (int e = 1; e <= p.groups; ++e) last = checked_offset(p, e, last);
-        s_last = last;
-    }
-    __syncthreads();
-    TO* c = static_cast<TO*>(p.c);
-    for (int t = blockIdx.x; t < p.rows; t += gridDim.x)
-        if (t < s_first || t >= s_last)
-            for (int j = threadIdx.x; j < p.n; j += 256) c[t * p.ldc + j] = from_f32<TO>(0.0f);
-}
 
 int dtype_bytes(int dtype) { return dtype == MFB_DTYPE_F32 ? 4 : 2; }
 
@@ -175,8 +19,10 @@ mfb_status_t validate_grouped(const mfb_grouped_desc* d, const int* offsets, con
     if (!d) return fail(MFB_EINVAL, "null grouped descriptor");
     if (d->groups < 0 || d->rows < 0 || d->n < 0 || d->k < 0)
         return fail(MFB_EINVAL, "grouped product dimensions must be non-negative");
-    if (d->groups > kMaxGroups)
-        return fail(MFB_EINVAL, "at most " + std::to_string(kMaxGroups) + " groups are supported");
+    if (std::max({d->rows, d->n, d->k}) > INT32_MAX - 65536)
+        return fail(MFB_EINVAL, "grouped product dimension exceeds the 32-bit limit");
+    if (d->groups > kGroupedMaxGroups)
+        return fail(MFB_EINVAL, "at most " + std::to_string(kGroupedMaxGroups) + " groups are supported");
     if (d->dtype < MFB_DTYPE_F32 || d->dtype > MFB_DTYPE_BF16) return fail(MFB_EINVAL, "invalid grouped operand type");
     if (d->out_dtype != d->dtype && d->out_dtype != MFB_DTYPE_F32)
         return fail(MFB_EINVAL, "the output of a grouped product has the operands' type or FP32");
@@ -221,32 +67,162 @@ mfb_status_t validate_grouped(const mfb_grouped_desc* d, const int* offsets, con
     return MFB_OK;
 }
 
-GroupedParams grouped_params(const mfb_grouped_desc& d, const int* offsets, const void* a, const void* b, void* c) {
-    return GroupedParams{offsets, d.groups, d.rows,    d.n,         d.k, d.lda, d.ldb,
-                         d.ldc,   d.stride, d.trans_b, d.zero_rest, a,   b,     c};
+// One instance of the kernel.
+struct GroupedEntry {
+    const void* fn;
+    int smem, threads, nt, cg;
+};
+
+template <class Cfg>
+GroupedEntry entry() {
+    return GroupedEntry{reinterpret_cast<const void*>(&grouped_tc_kernel<Cfg>), Cfg::kSmem, Cfg::kThreads, Cfg::NT, Cfg::CG};
 }
 
-template <typename T, typename TO>
-mfb_status_t launch_simple(const GroupedParams& p, cudaStream_t stream, bool right) {
-    const unsigned nx = static_cast<unsigned>((p.n + 63) / 64);
-    if (right) {
-        grouped_right_simple_kernel<T, TO><<<dim3(nx, (p.k + 63) / 64, p.groups), 256, 0, stream>>>(p);
-    } else {
-        if (p.groups > 0)
-            grouped_simple_kernel<T, TO><<<dim3(nx, (p.rows + 63) / 64 + p.groups), 256, 0, stream>>>(p);
-        if (p.zero_rest) grouped_rest_kernel<TO><<<4 * current_sm_count(), 256, 0, stream>>>(p);
+// Wide tiles on SM pairs, narrow ones on single SMs.
+template <int PLANES, bool RIGHT, bool M_MN, bool TMA>
+GroupedEntry entry_for(bool wide) {
+    if constexpr (PLANES == 1)
+        return wide ? entry<GroupedConfig<256, 2, 1, RIGHT, M_MN, TMA, 6>>() : entry<GroupedConfig<64, 1, 1, RIGHT, M_MN, TMA, 8>>();
+    else
+        return wide ? entry<GroupedConfig<128, 2, PLANES, RIGHT, M_MN, false, 3>>()
+                    : entry<GroupedConfig<64, 1, PLANES, RIGHT, M_MN, false, 3>>();
+}
+
+template <int PLANES, bool TMA>
+GroupedEntry entry_of(bool right, bool m_mn, bool wide) {
+    if (right) return entry_for<PLANES, true, true, TMA>(wide);
+    return m_mn ? entry_for<PLANES, false, true, TMA>(wide) : entry_for<PLANES, false, false, TMA>(wide);
+}
+
+// Raises the kernel's shared-memory limit once per device, and says how many of its workers (SMs or SM
+// pairs) fit on the device at once.
+mfb_status_t grouped_workers(const GroupedEntry& e, int device, int* out) {
+    static std::mutex mutex;
+    static std::map<std::pair<int, const void*>, int> cache;
+    std::lock_guard<std::mutex> lock(mutex);
+    auto it = cache.find({device, e.fn});
+    if (it != cache.end()) {
+        *out = it->second;
+        return MFB_OK;
     }
-    MFB_CUDA_TRY(cudaGetLastError(), "grouped product launch");
+    MFB_CUDA_TRY(cudaFuncSetAttribute(e.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, e.smem),
+                 "cudaFuncSetAttribute(grouped product)");
+    int workers = sm_count(device);
+    if (e.cg == 2) {
+        cudaLaunchConfig_t lc{};
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {2, 1, 1};
+        lc.gridDim = dim3(static_cast<unsigned>(2 * (workers / 2)));
+        lc.blockDim = dim3(static_cast<unsigned>(e.threads));
+        lc.dynamicSmemBytes = static_cast<size_t>(e.smem);
+        lc.attrs = &attr;
+        lc.numAttrs = 1;
+        MFB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&workers, e.fn, &lc), "cudaOccupancyMaxActiveClusters");
+        if (workers <= 0) return fail(MFB_EUNSUPPORTED, "no SM pair can host the grouped product");
+    }
+    cache[{device, e.fn}] = workers;
+    *out = workers;
     return MFB_OK;
 }
 
-mfb_status_t launch_grouped(const mfb_grouped_desc& d, const GroupedParams& p, cudaStream_t stream, bool right) {
-    if (d.dtype == MFB_DTYPE_F32) return launch_simple<float, float>(p, stream, right);
-    if (d.dtype == MFB_DTYPE_F16)
-        return d.out_dtype == MFB_DTYPE_F32 ? launch_simple<__half, float>(p, stream, right)
-                                            : launch_simple<__half, __half>(p, stream, right);
-    return d.out_dtype == MFB_DTYPE_F32 ? launch_simple<__nv_bfloat16, float>(p, stream, right)
-                                        : launch_simple<__nv_bfloat16, __nv_bfloat16>(p, stream, right);
+// Tensor map over `count` matrices of 16-bit elements, boxes of 64 columns.
+mfb_status_t encode_16bit(CUtensorMap* map, const void* base, long long rows, int cols, long long ld, long long count,
+                          long long stride, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(MFB_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
+                                static_cast<cuuint64_t>(count)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(count > 1 ? stride : ld) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+    const cuuint32_t step[3] = {1, 1, 1};
+    // The bits are copied as they are, FP16 or BF16.
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(MFB_ECUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string(static_cast<int>(r)) + ")");
+    return MFB_OK;
+}
+
+// The largest power of two up to 32 that divides the address and every stride in bytes.
+int common_alignment(const void* p, long long s0, long long s1) {
+    const unsigned long long v = reinterpret_cast<uintptr_t>(p) | static_cast<unsigned long long>(s0) |
+                                 static_cast<unsigned long long>(s1) | 32u;
+    return static_cast<int>(v & (~v + 1));
+}
+
+mfb_status_t launch_grouped(int device, const mfb_grouped_desc& d, cudaStream_t stream, const int* offsets,
+                            const void* a, const void* b, void* c, bool right) {
+    const int size = dtype_bytes(d.dtype);
+    const bool shared = right || d.groups <= 1 || d.stride == 0;  // B is one matrix
+    GroupedParams p{};
+    p.offsets = offsets;
+    p.groups = d.groups;
+    p.rows = d.rows;
+    p.n = d.n;
+    p.k = d.k;
+    p.ldc = d.ldc;
+    p.stride_c = right ? d.stride : 0;
+    p.c = c;
+    p.out_f32 = d.out_dtype == MFB_DTYPE_F32;
+    p.bf16 = d.dtype == MFB_DTYPE_BF16;
+    p.zero_rest = d.zero_rest;
+    p.wait_limit_ns = wait_limit_ns();
+    p.m_base = static_cast<const char*>(b);
+    p.n_base = static_cast<const char*>(a);
+    p.m_ld = d.ldb * static_cast<long long>(size);
+    p.n_ld = d.lda * static_cast<long long>(size);
+    p.m_stride = shared ? 0 : d.stride * size;
+    p.m_align = common_alignment(b, p.m_ld, p.m_stride);
+    p.n_align = common_alignment(a, p.n_ld, 0);
+    p.m_shared = shared;
+
+    const bool m_mn = !d.trans_b;
+    const bool tma = size == 2 && p.m_align >= 16 && p.n_align >= 16 && d.groups > 0 && d.k > 0 && d.rows > 0;
+    // Rows of C per matrix: few of them leave a wide tile mostly empty, and the weights are what costs.
+    const bool wide = (right ? d.k : d.rows / std::max(1, d.groups)) > 64;
+    const GroupedEntry e = size == 2 ? (tma ? entry_of<1, true>(right, m_mn, wide) : entry_of<1, false>(right, m_mn, wide))
+                           : d.precision == MFB_PRECISION_FP32 ? entry_of<3, false>(right, m_mn, wide)
+                                                               : entry_of<2, false>(right, m_mn, wide);
+    p.m_tiles = (d.n + 128 * e.cg - 1) / (128 * e.cg);
+    // An upper bound of the tiles: each group may have one that its rows do not fill.
+    const long long row_tiles = right ? static_cast<long long>(d.groups) * ((d.k + e.nt - 1) / e.nt)
+                                      : (d.rows + e.nt - 1) / e.nt + std::min(d.groups, d.rows);
+    if (row_tiles * p.m_tiles > 0x7fffffffLL) return fail(MFB_EINVAL, "problem has too many output tiles");
+
+    CUtensorMap maps[3] = {};
+    if (tma) {
+        if (right) {
+            MFB_TRY(encode_16bit(&maps[0], b, d.rows, d.n, d.ldb, 1, 0, 64));
+            MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, 64));
+            maps[2] = maps[1];
+        } else {
+            const long long b_rows = d.trans_b ? d.n : d.k;
+            const int b_cols = d.trans_b ? d.k : d.n;
+            MFB_TRY(encode_16bit(&maps[0], b, b_rows, b_cols, d.ldb, shared ? 1 : d.groups, d.stride, m_mn ? 64 : 128));
+            MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, e.nt / e.cg));
+            MFB_TRY(encode_16bit(&maps[2], a, d.rows, d.k, d.lda, 1, 0, 16));
+        }
+    }
+    int workers = 0;
+    MFB_TRY(grouped_workers(e, device, &workers));
+    // Without tiles the launch still clears the rows of no group.
+    const long long useful = std::max(row_tiles * p.m_tiles, d.zero_rest ? (d.rows + 7ll) / 8 : 1ll);
+    workers = static_cast<int>(std::min<long long>(workers, useful));
+    void* args[] = {&maps[0], &maps[1], &maps[2], &p};
+    cudaLaunchConfig_t lc{};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {2, 1, 1};
+    lc.gridDim = dim3(static_cast<unsigned>(e.cg * workers));
+    lc.blockDim = dim3(static_cast<unsigned>(e.threads));
+    lc.dynamicSmemBytes = static_cast<size_t>(e.smem);
+    lc.stream = stream;
+    lc.attrs = &attr;
+    lc.numAttrs = e.cg == 2 ? 1 : 0;
+    MFB_CUDA_TRY(cudaLaunchKernelExC(&lc, e.fn, args), "grouped product launch");
+    return MFB_OK;
 }
 
 }  // namespace
@@ -263,8 +239,7 @@ MFB_API mfb_status_t mfb_grouped_gemm(int device, mfb_stream_t stream, const mfb
     if (desc->rows == 0 || desc->n == 0) return MFB_OK;
     DeviceGuard guard;
     MFB_TRY(select_device(device));
-    return launch_grouped(*desc, grouped_params(*desc, offsets, a, b, c), reinterpret_cast<cudaStream_t>(stream),
-                          false);
+    return launch_grouped(device, *desc, reinterpret_cast<cudaStream_t>(stream), offsets, a, b, c, false);
 }
 
 MFB_API mfb_status_t mfb_grouped_gemm_bwd_right(int device, mfb_stream_t stream, const mfb_grouped_desc* desc,
@@ -274,8 +249,7 @@ MFB_API mfb_status_t mfb_grouped_gemm_bwd_right(int device, mfb_stream_t stream,
     if (desc->groups == 0 || desc->k == 0 || desc->n == 0) return MFB_OK;
     DeviceGuard guard;
     MFB_TRY(select_device(device));
-    return launch_grouped(*desc, grouped_params(*desc, offsets, a, b, c), reinterpret_cast<cudaStream_t>(stream),
-                          true);
+    return launch_grouped(device, *desc, reinterpret_cast<cudaStream_t>(stream), offsets, a, b, c, true);
 }
 
 }  // extern "C"

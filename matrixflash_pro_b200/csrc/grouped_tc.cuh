@@ -1,0 +1,642 @@
+// The tcgen05 kernel of the products grouped by expert.
+//
+// One accumulator tile D (M x N) has output columns on its M side and output rows on its N side:
+//   forward:  D[f, t] = sum_k  op(B_e)[k, f] A[t, k]   N side: rows t of one group
+//   gradient: D[j, i] = sum_t  B[t, j]       A[t, i]   contraction over the rows t of one group
+// so a TMEM lane is an output column and an accumulator column an output row. Weights always fill the M
+// side, whatever a group's size; the N side of an MMA may be any multiple of 16 (32 on SM pairs), so a
+// group of 3 rows costs an MMA of 16 or 32 columns and not a tile of 128 rows.
+//
+// Group sizes are device data. Every CTA scans the offsets once into shared memory (tiles before each
+// group), and its roles walk the same tile sequence, dealt out round-robin to the persistent workers.
+//
+// 16-bit operands whose rows TMA can address come by TMA, 64 of the contraction deep, 128-byte swizzle
+// (K-major tiles one box or boxes of 16 rows; MN-major tiles boxes of 64 columns). All others (FP32, odd
+// strides) come by eight loader warps that read global memory into registers and write the same layout:
+// 16-bit values as they are, FP32 as PLANES BF16 terms x = h + m + l (h cut, m and l rounded; exact with
+// three). Products hh, hm, mh, mm, hl, lh are kept (six MMAs per step, 1/6 of the BF16 rate); what is left
+// out is below 2^-21 of |a b|. Two terms (TF32 precision) keep hh, hm, mh.
+//
+// The tensor core adds with truncation, so strict FP32 restarts the accumulator every 64 of the
+// contraction and the epilogue warps add the chunks in registers, rounding to nearest.
+#pragma once
+
+#include "mfb_device.cuh"
+#include "mfb_internal.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace mfb {
+
+constexpr int kGroupedMaxGroups = 1024;
+constexpr int kGroupedDepth = 64;  // contraction per stage: one 128-byte row of 16-bit values
+
+struct GroupedParams {
+    const int* offsets;
+    int groups, rows;       // rows of A
+    int n, k;               // C is .. x n; k: contraction (forward) or rows of each C_e (gradient)
+    long long ldc, stride_c;
+    void* c;
+    int out_f32, bf16, zero_rest;
+    int m_tiles;            // tiles along the M side (n)
+    uint64_t wait_limit_ns;
+    // Operands for the loader warps: M side (B) and N side (A). align: bytes that every row start is a multiple of.
+    const char* m_base;
+    const char* n_base;
+    long long m_ld, m_stride, n_ld;  // bytes
+    int m_align, n_align;
+    int m_shared;  // all groups share one matrix: the tensor map has one
+};
+
+template <int NT_, int CG_, int PLANES_, bool RIGHT_, bool M_MN_, bool TMA_, int STAGES_>
+struct GroupedConfig {
+    static constexpr int NT = NT_, CG = CG_, PLANES = PLANES_, STAGES = STAGES_;
+    static constexpr bool RIGHT = RIGHT_, TMA = TMA_;
+    static constexpr bool M_MN = RIGHT_ || M_MN_;  // M side stored MN-major
+    static constexpr bool N_MN = RIGHT_;           // N side stored MN-major
+    static constexpr int ES = PLANES == 1 ? 2 : 4;  // bytes of an operand element in memory
+    static constexpr int BM = 128 * CG;
+    static constexpr int NTC = NT / CG;  // N-side rows of a CTA
+    static constexpr int kMPlane = 128 * 128, kNPlane = NTC * 128;
+    static constexpr int kMBytes = PLANES * kMPlane, kNBytes = PLANES * kNPlane;
+    static constexpr int kStage = kMBytes + kNBytes;
+    static constexpr int kBarriers = STAGES * kStage;
+    static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 5) + 16;
+    static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
+    static constexpr int kLoaders = TMA ? 1 : 8;  // warps
+    static constexpr int kMmaWarp = kLoaders, kFixWarp = kLoaders + 1;
+    static constexpr int kEpiWarp0 = TMA && RIGHT ? kLoaders + 2 : kLoaders + 1;
+    static constexpr int kEpiWarps = 8;
+    static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+    static constexpr int kTmemCols = 2 * NT;
+    static constexpr int kGranule = 16 * CG;  // N of an MMA is a multiple of this
+    // Arrivals that complete a filled stage, besides the bytes of TMA copies.
+    static constexpr int kFullCount = !TMA ? CG * kLoaders : RIGHT ? CG : 1;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+    static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512 && kTmemCols >= 32, "TMEM allocation");
+    static_assert(!N_MN || NTC % 64 == 0, "MN-major boxes are 64 columns");
+};
+
+struct GroupedTile {
+    int e;
+    int f0;          // first output column of the tile
+    int r0, r1;      // output rows [r0, r1)
+    int cols;        // N of the MMAs
+    int t0, t1;      // gradient: rows contracted over
+    int kb;          // stages
+};
+
+template <class Cfg>
+struct GroupedTiles {
+    const GroupedParams& p;
+    const int* offset;      // [groups + 1], clamped
+    const int* first_tile;  // [groups + 1]
+    int tile, step, e;
+
+    __device__ GroupedTiles(const GroupedParams& p_, const int* o, const int* f, int worker, int workers)
+        : p(p_), offset(o), first_tile(f), tile(worker - workers), step(workers), e(0) {}
+
+    __device__ bool next(GroupedTile& t) {
+        tile += step;
+        if (tile >= first_tile[p.groups]) return false;
+        while (tile >= first_tile[e + 1]) ++e;
+        const int i = tile - first_tile[e];
+        t.e = e;
+        t.t0 = offset[e];
+        t.t1 = offset[e + 1];
+        // Tiles that share M-side data follow each other. The output rows are dealt out evenly: 300 rows are
+        // 160 + 140, not 256 + 44 (every tile is left some, since (tiles - 1) NT < rows and each <= NT).
+        const int rows = Cfg::RIGHT ? p.k : t.t1 - t.t0;
+        const int tiles = (rows + Cfg::NT - 1) / Cfg::NT;
+        const int each = ((rows + tiles - 1) / tiles + Cfg::kGranule - 1) / Cfg::kGranule * Cfg::kGranule;
+        const int ri = i % tiles * each;
+        const int left = min(each, rows - ri);
+        t.f0 = i / tiles * Cfg::BM;
+        t.r0 = (Cfg::RIGHT ? 0 : t.t0) + ri;
+        t.r1 = t.r0 + left;
+        t.cols = (left + Cfg::kGranule - 1) / Cfg::kGranule * Cfg::kGranule;
+        t.kb = ((Cfg::RIGHT ? t.t1 - t.t0 : p.k) + kGroupedDepth - 1) / kGroupedDepth;
+        return true;
+    }
+};
+
+__device__ __forceinline__ void grouped_store(const GroupedParams& p, long long at, float v) {
+    if (p.out_f32) static_cast<float*>(p.c)[at] = v;
+    else if (p.bf16) static_cast<__nv_bfloat16*>(p.c)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p.c)[at] = __float2half_rn(v);
+}
+
+// Eight consecutive elements of a row in global memory; zeros outside [.., rows) x [.., cols).
+template <int ES>
+struct GroupedChunk {
+    uint32_t w[2 * ES];  // ES 2: four words of two values; ES 4: eight FP32 values
+
+    __device__ __forceinline__ void load(const char* base, long long ld, int align, int row, int rows, int col,
+                                         int cols) {
+#pragma unroll
+        for (int i = 0; i < 2 * ES; ++i) w[i] = 0;
+        if (row >= rows || col >= cols) return;
+        const char* src = base + row * ld + static_cast<long long>(col) * ES;
+        if (col + 8 <= cols) {
+            if (align >= 16) {
+#pragma unroll
+                for (int i = 0; i < ES / 2; ++i) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+                    w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+                }
+                return;
+            }
+            if (align >= 4) {
+#pragma unroll
+                for (int i = 0; i < 2 * ES; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+                return;
+            }
+            if (ES == 2) {  // rows start at any even address
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+                if (reinterpret_cast<uintptr_t>(src) & 2) {
+                    const uint32_t first = __ldg(h), last = __ldg(h + 7);
+                    uint32_t v[3];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) v[i] = __ldg(reinterpret_cast<const uint32_t*>(h + 1) + i);
+                    w[0] = first | v[0] << 16;
+                    w[1] = v[0] >> 16 | v[1] << 16;
+                    w[2] = v[1] >> 16 | v[2] << 16;
+                    w[3] = v[2] >> 16 | last << 16;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+                }
+                return;
+            }
+        }
+        const int count = min(8, cols - col);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= count) continue;
+            if (ES == 2)
+                w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + i)) << (16 * (i % 2));
+            else
+                w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+        }
+    }
+
+    // Into 16 bytes of each plane at shared address `to`.
+    template <int PLANES>
+    __device__ __forceinline__ void store(uint32_t to, int plane_bytes) const {
+        if constexpr (PLANES == 1) {
+            st(to, w[0], w[1], w[2], w[3]);
+        } else {
+            uint32_t t[PLANES][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float lo = __uint_as_float(w[2 * i]), hi = __uint_as_float(w[2 * i + 1]);
+                asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(t[0][i]) : "f"(hi), "f"(lo));
+#pragma unroll
+                for (int pl = 1; pl < PLANES; ++pl) {
+                    lo -= __uint_as_float(t[pl - 1][i] << 16);
+                    hi -= __uint_as_float(t[pl - 1][i] & 0xffff0000u);
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(t[pl][i]) : "f"(hi), "f"(lo));
+                }
+            }
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) st(to + pl * plane_bytes, t[pl][0], t[pl][1], t[pl][2], t[pl][3]);
+        }
+    }
+
+    __device__ __forceinline__ static void st(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    }
+};
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1)
+    grouped_tc_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n,
+                      const __grid_constant__ CUtensorMap map_n16, const GroupedParams p) {
+    constexpr int NT = Cfg::NT, CG = Cfg::CG, PLANES = Cfg::PLANES, STAGES = Cfg::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kBarriers);  // used in the leader
+    uint64_t* empty_bar = full_bar + STAGES;
+    uint64_t* tail_bar = empty_bar + STAGES;  // a stage whose last rows are still to be cleared
+    uint64_t* acc_full_bar = tail_bar + STAGES;
+    uint64_t* acc_empty_bar = acc_full_bar + 2;  // used in the leader
+    uint64_t* drain_bar = acc_empty_bar + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* offset = reinterpret_cast<int*>(smem + Cfg::kTables);
+    int* first_tile = offset + kGroupedMaxGroups + 1;
+
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
+    const bool leader = rank == 0;
+    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full_bar[s], Cfg::kFullCount);
+            mbar_init(&empty_bar[s], 1);
+            mbar_init(&tail_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full_bar[b], 1);
+            mbar_init(&acc_empty_bar[b], CG * Cfg::kEpiWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == Cfg::kMmaWarp) {
+        if (CG == 2) {
+            tmem_alloc_pair(tmem_slot, Cfg::kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, Cfg::kTmemCols);
+            tmem_relinquish();
+        }
+    }
+    if (warp == Cfg::kEpiWarp0) {
+        // Clamped offsets (running maximum) and the tiles in front of each group, 32 groups at a time.
+        int floor = 0, before = 0;
+        for (int base = 0; base <= p.groups; base += 32) {
+            const int i = base + lane;
+            const int raw = i <= p.groups ? p.offsets[i] : 0;
+            int v = min(max(raw, 0), p.rows);
+            if (i > p.groups) v = 0;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int o = __shfl_up_sync(~0u, v, d);
+                if (lane >= d) v = max(v, o);
+            }
+            v = max(v, floor);
+            if (i <= p.groups) {
+                offset[i] = v;
+                if (v != raw && worker == 0 && leader) atomicOr(&g_status, kStatusBadIndex);
+            }
+            int prev = __shfl_up_sync(~0u, v, 1);
+            if (lane == 0) prev = floor;
+            floor = __shfl_sync(~0u, v, 31);
+            // tiles of group i - 1, which ends here
+            const int rows = Cfg::RIGHT ? p.k : v - prev;
+            int tiles = i >= 1 && i <= p.groups ? (rows + NT - 1) / NT * p.m_tiles : 0;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int o = __shfl_up_sync(~0u, tiles, d);
+                if (lane >= d) tiles += o;
+            }
+            tiles += before;
+            if (i <= p.groups) first_tile[i] = tiles;
+            before = __shfl_sync(~0u, tiles, 31);
+        }
+    }
+    if (Cfg::TMA && warp == 0 && lane == 0) {
+        tma_prefetch_desc(&map_m);
+        tma_prefetch_desc(&map_n);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint64_t limit = p.wait_limit_ns;
+    GroupedTiles<Cfg> work(p, offset, first_tile, worker, workers);
+    GroupedTile t;
+
+    auto give_up = [&](uint32_t bits) {
+        report_status(bits, abort_flag);
+        if (CG == 2) st_cluster_u32(map_to_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1), 1);
+    };
+    auto leader_bar = [&](uint64_t* bar) { return map_to_cta(smem_u32(bar), 0); };
+    auto arrive_leader = [&](uint64_t* bar) {
+        if (CG == 2) mbar_arrive_cluster(leader_bar(bar));
+        else mbar_arrive(bar);
+    };
+
+    if (Cfg::TMA && warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            while (ok && work.next(t)) {
+                const int half = t.cols / CG;  // N-side rows of this CTA
+                const int n_rows = Cfg::N_MN ? (half + 63) / 64 * 64 : half;
+                const uint32_t bytes = Cfg::kMPlane + n_rows * 128;
+                const int f = t.f0 + 128 * rank, r = t.r0 + half * rank;
+                for (int kb = 0; kb < t.kb; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait_bounded(&empty_bar[s], ((it / STAGES) & 1) ^ 1, limit, abort_flag)) {
+                        give_up(kStatusTimeoutProducer);
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* m_tile = smem + s * Cfg::kStage;
+                    uint8_t* n_tile = m_tile + Cfg::kMBytes;
+                    const int d0 = (Cfg::RIGHT ? t.t0 : 0) + kb * kGroupedDepth;
+                    const bool tail = Cfg::RIGHT && d0 + kGroupedDepth > t.t1;
+                    uint64_t* bar = tail ? &tail_bar[s] : &full_bar[s];
+                    if (tail) mbar_arrive_expect_tx(bar, bytes);
+                    else if (leader) mbar_arrive_expect_tx(bar, CG * bytes);
+                    else if (Cfg::kFullCount == CG) arrive_leader(bar);
+                    const uint32_t to = map_to_cta(smem_u32(bar), tail ? rank : 0);
+                    auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
+                        if (CG == 2) tma_load_3d_pair(dst, map, to, x, y, z);
+                        else tma_load_3d(dst, map, bar, x, y, z);
+                    };
+                    const int z = Cfg::RIGHT || p.m_shared ? 0 : t.e;
+                    if (Cfg::M_MN) {
+                        load(m_tile, &map_m, f, d0, z);
+                        load(m_tile + 8192, &map_m, f + 64, d0, z);
+                    } else {
+                        load(m_tile, &map_m, d0, f, z);
+                    }
+                    if (Cfg::N_MN) {
+                        for (int b = 0; b < n_rows / 64; ++b) load(n_tile + b * 8192, &map_n, r + 64 * b, d0, 0);
+                    } else if (half == Cfg::NTC) {
+                        load(n_tile, &map_n, d0, r, 0);
+                    } else {
+                        for (int b = 0; b < half / 16; ++b) load(n_tile + b * 2048, &map_n16, d0, r + 16 * b, 0);
+                    }
+                }
+            }
+            // Drain: the copies in flight land (their stages are consumed) before this CTA ends.
+            for (int j = it - STAGES < 0 ? 0 : it - STAGES; j < it; ++j) {
+                if (!mbar_wait_drain(&empty_bar[j % STAGES], (j / STAGES) & 1, limit)) {
+                    report_status(kStatusTimeoutDrain, nullptr);
+                    break;
+                }
+            }
+        }
+    } else if (!Cfg::TMA && warp < Cfg::kLoaders) {
+        // ------------------------------------------------------------ loader warps
+        constexpr int ES = Cfg::ES;
+        constexpr int kThreads = 32 * Cfg::kLoaders;
+        constexpr int kM = 1024 / kThreads, kN = (Cfg::NTC * 8 + kThreads - 1) / kThreads;  // chunks per thread
+        GroupedChunk<ES> cm[kM], cn[kN];
+        const int id = threadIdx.x;
+        int it = 0;
+        bool ok = true;
+        while (ok && work.next(t)) {
+            const int half = t.cols / CG;
+            const int f = t.f0 + 128 * rank, r = t.r0 + half * rank;
+            const char* mb = p.m_base + (Cfg::RIGHT ? 0 : t.e * p.m_stride);
+            const int depth_end = Cfg::RIGHT ? t.t1 : p.k;
+            const int r_end = Cfg::RIGHT ? p.k : t.t1;
+            auto load_m = [&](int kb) {
+                const int d0 = (Cfg::RIGHT ? t.t0 : 0) + kb * kGroupedDepth;
+#pragma unroll
+                for (int i = 0; i < kM; ++i) {
+                    const int q = i * kThreads + id;
+                    if (Cfg::M_MN)
+                        cm[i].load(mb, p.m_ld, p.m_align, d0 + q / 16, depth_end, f + q % 16 * 8, p.n);
+                    else
+                        cm[i].load(mb, p.m_ld, p.m_align, f + q / 8, p.n, d0 + q % 8 * 8, depth_end);
+                }
+            };
+            auto load_n = [&](int kb) {
+                const int d0 = (Cfg::RIGHT ? t.t0 : 0) + kb * kGroupedDepth;
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    const int q = i * kThreads + id;
+                    constexpr int kRow = Cfg::NTC / 8;  // chunks of an MN-major row
+                    if (Cfg::N_MN)
+                        cn[i].load(p.n_base, p.n_ld, p.n_align, d0 + q / kRow, depth_end, r + q % kRow * 8,
+                                   q % kRow * 8 < half ? r_end : 0);
+                    else
+                        cn[i].load(p.n_base, p.n_ld, p.n_align, r + q / 8, q / 8 < half ? r_end : 0, d0 + q % 8 * 8,
+                                   depth_end);
+                }
+            };
+            if (t.kb > 0) {
+                load_m(0);
+                load_n(0);
+            }
+            for (int kb = 0; kb < t.kb; ++kb, ++it) {
+                const int s = it % STAGES;
+                ok = mbar_wait_bounded(&empty_bar[s], ((it / STAGES) & 1) ^ 1, limit, abort_flag);
+                ok = __all_sync(~0u, ok);
+                if (!ok) {
+                    if (lane == 0) give_up(kStatusTimeoutProducer);
+                    break;
+                }
+                const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
+                const uint32_t n_tile = m_tile + Cfg::kMBytes;
+#pragma unroll
+                for (int i = 0; i < kM; ++i) {
+                    const int q = i * kThreads + id;
+                    const int row = Cfg::M_MN ? q / 16 : q / 8, c = q % 8, box = Cfg::M_MN ? q % 16 / 8 : 0;
+                    cm[i].template store<PLANES>(m_tile + box * 8192 + row * 128 + ((c ^ (row & 7)) << 4), Cfg::kMPlane);
+                }
+                if (kb + 1 < t.kb) load_m(kb + 1);
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    const int q = i * kThreads + id;
+                    constexpr int kRow = Cfg::NTC / 8;
+                    const int row = Cfg::N_MN ? q / kRow : q / 8, c = q % 8, box = Cfg::N_MN ? q % kRow / 8 : 0;
+                    if ((Cfg::NTC * 8) % kThreads == 0 || q < Cfg::NTC * 8)
+                        cn[i].template store<PLANES>(n_tile + box * 8192 + row * 128 + ((c ^ (row & 7)) << 4),
+                                                     Cfg::kNPlane);
+                }
+                if (kb + 1 < t.kb) load_n(kb + 1);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&full_bar[s]);
+            }
+        }
+    } else if (warp == Cfg::kMmaWarp) {
+        // ------------------------------------------------------------ MMA issuer (leader)
+        if (lane == 0 && leader) {
+            int it = 0, buf = 0;
+            bool ok = true;
+            while (ok && work.next(t)) {
+                const uint32_t idesc =
+                    umma_idesc_f16(Cfg::BM, t.cols, Cfg::M_MN, Cfg::N_MN, PLANES > 1 ? 1 : p.bf16);
+                uint32_t d_tmem = 0, acc = 0;
+                for (int kb = 0; kb < t.kb; ++kb, ++it) {
+                    if (kb == 0 || PLANES == 3) {
+                        const int b = buf & 1;
+                        if (!mbar_wait_bounded(&acc_empty_bar[b], ((buf >> 1) & 1) ^ 1, limit, abort_flag)) {
+                            give_up(kStatusTimeoutMma);
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        d_tmem = tmem_base + b * NT;
+                        acc = 0;
+                    }
+                    const int s = it % STAGES;
+                    if (!mbar_wait_bounded(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
+                        give_up(kStatusTimeoutMma);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage);
+                    const uint32_t n_addr = m_addr + Cfg::kMBytes;
+                    auto m_desc = [&](int pl, int ks) {
+                        const uint32_t a = m_addr + pl * Cfg::kMPlane;
+                        return Cfg::M_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
+                                         : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
+                    };
+                    auto n_desc = [&](int pl, int ks) {
+                        const uint32_t a = n_addr + pl * Cfg::kNPlane;
+                        return Cfg::N_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
+                                         : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
+                    };
+                    auto mma = [&](int mp, int np, int ks) {
+                        if (CG == 2) umma_f16_pair(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
+                        else umma_f16(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
+                        acc = 1;
+                    };
+                    // The small products of all steps first: every addition truncates relative to what the
+                    // accumulator holds, so only the last four cut at the sum's own size.
+                    constexpr int kTerms = PLANES == 3 ? 6 : PLANES == 2 ? 3 : 1;
+                    constexpr int kMTerm[6] = {2, 0, 1, 1, 0, 0}, kNTerm[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+                    for (int i = 6 - kTerms; i < 6; ++i)
+#pragma unroll
+                        for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                    if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
+                    else umma_commit(&empty_bar[s]);
+                    if (PLANES == 3 || kb == t.kb - 1) {
+                        if (CG == 2) umma_commit_pair(&acc_full_bar[buf & 1], 0x3);
+                        else umma_commit(&acc_full_bar[buf & 1]);
+                        ++buf;
+                    }
+                }
+            }
+            if (CG == 2) umma_commit_pair(drain_bar, 0x1);
+            else umma_commit(drain_bar);
+            if (!mbar_wait_drain(drain_bar, 0, limit)) report_status(kStatusTimeoutDrain, nullptr);
+        }
+    } else if (Cfg::TMA && Cfg::RIGHT && warp == Cfg::kFixWarp) {
+        // ------------------------------------------------------------ clears the rows behind a group
+        // The last stage of a contraction over a group's rows holds rows of the next group (or NaN of a
+        // buffer's spare rows): both operands' tails become 0 before the MMA may read them.
+        int it = 0;
+        uint32_t phases = 0;  // parity of each stage's tail barrier
+        bool ok = true;
+        while (ok && work.next(t)) {
+            const int valid = (t.t1 - t.t0) % kGroupedDepth;
+            it += t.kb;
+            if (valid == 0) continue;
+            const int s = (it - 1) % STAGES;
+            ok = mbar_wait_bounded(&tail_bar[s], (phases >> s) & 1, limit, abort_flag);
+            ok = __all_sync(~0u, ok);
+            if (!ok) {
+                if (lane == 0) give_up(kStatusTimeoutProducer);
+                break;
+            }
+            phases ^= 1u << s;
+            const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
+            const int boxes = (t.cols / CG + 63) / 64;
+            for (int b = 0; b < 2 + boxes; ++b) {
+                const uint32_t box = m_tile + (b < 2 ? b * 8192 : Cfg::kMBytes + (b - 2) * 8192);
+                for (int at = valid * 128 + lane * 16; at < 8192; at += 512) GroupedChunk<2>::st(box + at, 0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_leader(&full_bar[s]);
+        }
+    } else if (warp >= Cfg::kEpiWarp0) {
+        // ------------------------------------------------------------ epilogue
+        const int quarter = warp & 3;                    // TMEM lanes of this warp
+        const int part = (warp - Cfg::kEpiWarp0) >> 2;   // which of every two 16-column chunks
+        const uint32_t acc_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        int buf = 0;
+        bool ok = true;
+        while (ok && work.next(t)) {
+            const int f = t.f0 + 128 * rank + quarter * 32 + lane;
+            const long long at = (Cfg::RIGHT ? t.e * p.stride_c : 0) + t.r0 * p.ldc + f;
+            const int rows = f < p.n ? t.r1 - t.r0 : 0;  // this lane's column of each row
+            auto store = [&](int q, const float (&v)[16]) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (q * 16 + j < rows) grouped_store(p, at + (q * 16 + j) * p.ldc, v[j]);
+            };
+            if (t.kb == 0) {
+                const float zero[16] = {};
+                for (int q = part; q * 16 < t.cols; q += 2) store(q, zero);
+                continue;
+            }
+            constexpr int kChunks = NT / 32;
+            if constexpr (PLANES == 3) {
+                float sum[kChunks][16];
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[i][j] = 0.0f;
+                for (int kb = 0; kb < t.kb; ++kb, ++buf) {
+                    const int b = buf & 1;
+                    ok = mbar_wait_bounded(&acc_full_bar[b], (buf >> 1) & 1, limit, abort_flag);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i) {
+                        const int q = 2 * i + part;
+                        if (q * 16 < t.cols) {
+                            uint32_t v[16];
+                            tmem_ld_32x32b_x16(acc_base + b * NT + q * 16, v);
+                            tmem_ld_wait();
+                            tmem_regs_ready(v);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sum[i][j] += __uint_as_float(v[j]);
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_leader(&acc_empty_bar[b]);
+                }
+                if (ok) {
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
+                        if ((2 * i + part) * 16 < t.cols) store(2 * i + part, sum[i]);
+                }
+            } else {
+                const int b = buf & 1;
+                ok = mbar_wait_bounded(&acc_full_bar[b], (buf >> 1) & 1, limit, abort_flag);
+                ok = __all_sync(~0u, ok);
+                if (ok) {
+                    tc_fence_after();
+                    for (int q = part; q * 16 < t.cols; q += 2) {
+                        uint32_t v[16];
+                        tmem_ld_32x32b_x16(acc_base + b * NT + q * 16, v);
+                        tmem_ld_wait();
+                        tmem_regs_ready(v);
+                        float x[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]);
+                        store(q, x);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_leader(&acc_empty_bar[b]);
+                    ++buf;
+                }
+            }
+            if (!ok && lane == 0) give_up(kStatusTimeoutEpilogue);
+        }
+        if (!Cfg::RIGHT && p.zero_rest) {
+            // Rows of no group: in front of the first and behind the last one.
+            const int first = offset[0], last = offset[p.groups], rest = first + p.rows - last;
+            const int id = (blockIdx.x * Cfg::kEpiWarps + warp - Cfg::kEpiWarp0), ids = gridDim.x * Cfg::kEpiWarps;
+            for (int i = id; i < rest; i += ids) {
+                const long long row = i < first ? i : last + (i - first);
+                for (int j = lane; j < p.n; j += 32) grouped_store(p, row * p.ldc + j, 0.0f);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();  // both CTAs are done with each other's barriers and TMEM
+    if (warp == Cfg::kMmaWarp) {
+        tc_fence_after();
+        if (CG == 2) tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+        else tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+}
+
+}  // namespace mfb

@@ -34,7 +34,7 @@ from .errors import InvalidArgumentError, ShapeMismatchError
 from .gemm import GemmPrecision, checked_dim
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_MAX_GROUPS = 4096
+_MAX_GROUPS = 1024
 
 
 def _stream_of(device: torch.device, stream) -> int:

@@ -58,7 +58,7 @@ A, B, C, O = 0x100000, 0x200000, 0x300000, 0x400000
 
 @pytest.mark.parametrize("kw,needle", [
     (dict(groups=-1), "non-negative"), (dict(rows=-1), "non-negative"), (dict(n=-2), "non-negative"),
-    (dict(groups=4097), "4096"), (dict(dtype=3), "type"), (dict(dtype=1, out_dtype=2), "type"),
+    (dict(groups=1025), "1024"), (dict(dtype=3), "type"), (dict(dtype=1, out_dtype=2), "type"),
     (dict(precision=2), "precision"), (dict(trans_b=2), "trans_b"), (dict(zero_rest=-1), "zero_rest"),
     (dict(lda=3), "lda"), (dict(ldb=4), "ldb"), (dict(trans_b=1, ldb=3), "ldb"), (dict(ldc=4), "ldc"),
     (dict(stride=-1), "stride"),
