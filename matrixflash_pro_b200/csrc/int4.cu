@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace mfb {
@@ -137,17 +139,21 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const Int4Params p
 // ------------------------------------------------------------------------------------
 // y[r, i] = sum over groups of s[i, G] * sum_{j in G} (q - z)[i, j] x[r, j].
 //
-// The codes are read once and everything else fits beside that: a warp takes 16 * MT output rows and 128
-// columns at a time (16 bytes of codes per row and lane, four lanes to a row), turns codes into the exact
-// 16-bit integers q - z and feeds them to m16n8k16 MMAs as A, with up to 8 * RT rows of x as B. A group's sum
-// is an FP32 accumulator, its scale one FMA per accumulator. FP32 rows enter as three BF16 terms (exact),
-// added into the same accumulator, small ones first.
+// The codes are read once and everything else fits beside that: a warp takes 16 output rows and 128 columns
+// at a time (16 bytes of codes per row and lane, four lanes to a row), turns codes into the exact 16-bit
+// integers q - z and feeds them to m16n8k16 MMAs as A, with up to 8 * RT rows of x as B. A group's sum is an
+// FP32 accumulator, its scale one FMA per accumulator. FP32 rows enter as three BF16 terms (exact), added into
+// the same accumulator, small ones first.
 //
 // Which columns meet in one MMA step is free as long as A and B agree, so a lane's word of eight codes serves two
 // steps as it lies: (word >> 4 i) & 0x000f000f holds codes i and i + 4. For groups of 64 and 32 the four lanes of
 // a row exchange words first, so that all columns of a step share one scale.
 //
-// The 8 warps of a block take every eighth chunk of the same rows and add up in shared memory in a fixed order.
+// One block of 16 warps per SM takes an even share of the 16-row tiles. Its warps split the columns (KW warps,
+// every KW-th chunk each) and, where there are fewer chunks than warps, the tiles. A warp goes chunk by chunk
+// through the tiles, so a chunk of x is loaded and laid out once for all of them; codes and scales of the next
+// tiles are in flight in registers meanwhile. Sums wait in shared memory, a slot per tile, warp and lane, and are
+// added up in a fixed order at the end.
 
 template <typename T>
 struct Int4Math {  // FP16
@@ -241,52 +247,50 @@ __device__ __forceinline__ void load_x8(const T* row, int j, int k, bool vec, ui
     }
 }
 
-// A chunk's codes, scales and zero points for the 2 * MT rows of a lane.
-template <typename TS, int GROUP, int MT>
-struct Int4Chunk {
+// Codes, scales and zero points of one tile and chunk: rows g and g + 8 of this lane.
+template <typename TS, int GROUP>
+struct Int4Item {
     static constexpr int kGroups = 128 / GROUP;
-    uint4 w[MT][2];
-    TS s[MT][2][kGroups];
-    uint32_t z[MT][2];  // one byte per group
+    uint4 w[2];
+    TS s[2][kGroups];
+    uint32_t z[2];  // one byte per group
 
+    // vec: whole chunks of groups, aligned.
     __device__ __forceinline__ void load(const Int4Params& p, long long row0, int n_left, int chunk, int lane, bool vec) {
         const int byte = chunk * 64 + lane % 4 * 16;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int h = 0; h < 2; ++h) {
+            const long long row = row0 + min(h * 8 + lane / 4, n_left - 1);  // rows past the end repeat the last
+            w[h] = make_uint4(0, 0, 0, 0);
+            if (byte < p.row_bytes)
+                asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[h].x), "=r"(w[h].y), "=r"(w[h].z), "=r"(w[h].w)
+                             : "l"(p.packed + row * p.row_bytes + byte));
+            const long long at = row * p.groups + chunk * kGroups;
+            const TS* sp = static_cast<const TS*>(p.scales) + at;
+            z[h] = 0x08080808u;
+            if (vec) {
+                struct alignas(sizeof(TS) * kGroups) Vec {
+                    TS v[kGroups];
+                };
+                const Vec v = *reinterpret_cast<const Vec*>(sp);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const long long row = row0 + min(mt * 16 + h * 8 + lane / 4, n_left - 1);  // rows past the end repeat the last
-                const unsigned char* src = p.packed + row * p.row_bytes + byte;
-                w[mt][h] = make_uint4(0, 0, 0, 0);
-                if (byte < p.row_bytes)
-                    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(w[mt][h].x), "=r"(w[mt][h].y), "=r"(w[mt][h].z), "=r"(w[mt][h].w)
-                                 : "l"(src));
-                const long long at = row * p.groups + chunk * kGroups;
-                const TS* sp = static_cast<const TS*>(p.scales) + at;
-                z[mt][h] = 0x08080808u;
-                if (vec) {  // whole chunks of groups, aligned
-                    struct alignas(sizeof(TS) * kGroups) Vec {
-                        TS v[kGroups];
-                    };
-                    const Vec v = *reinterpret_cast<const Vec*>(sp);
+                for (int i = 0; i < kGroups; ++i) s[h][i] = v.v[i];
+                if (p.zeros) {
+                    if (kGroups == 4) z[h] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
+                    else if (kGroups == 2) z[h] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
+                    else z[h] = __ldg(p.zeros + at);
+                }
+            } else {
+                if (p.zeros) z[h] = 0;
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i) s[mt][h][i] = v.v[i];
-                    if (p.zeros) {
-                        if (kGroups == 4) z[mt][h] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
-                        else if (kGroups == 2) z[mt][h] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
-                        else z[mt][h] = __ldg(p.zeros + at);
-                    }
-                } else {
-                    if (p.zeros) z[mt][h] = 0;
-#pragma unroll
-                    for (int i = 0; i < kGroups; ++i) {
-                        const bool in = chunk * kGroups + i < p.groups;
-                        s[mt][h][i] = in ? sp[i] : from_f32<TS>(0.0f);
-                        if (p.zeros && in) z[mt][h] |= static_cast<uint32_t>(__ldg(p.zeros + at + i)) << (8 * i);
-                    }
+                for (int i = 0; i < kGroups; ++i) {
+                    const bool in = chunk * kGroups + i < p.groups;
+                    s[h][i] = in ? sp[i] : from_f32<TS>(0.0f);
+                    if (p.zeros && in) z[h] |= static_cast<uint32_t>(__ldg(p.zeros + at + i)) << (8 * i);
                 }
             }
+        }
     }
 };
 
@@ -314,160 +318,249 @@ __device__ __forceinline__ int slot_column(int t, int i) {
     return 32 * i + 8 * t;
 }
 
-constexpr int kGemvWarps = 8;
+constexpr int kGemvWarps = 16;
+constexpr int kGemvSlots = 128;  // 16-row tiles times warps along k whose sums one block holds at a time
+constexpr int kGemvSmem = kGemvSlots * 32 * 16;
 
-// blockIdx.x: 16 * MT output rows. With ids, blockIdx.y is a row of x, and the block serves all rows of that row's
-// expert if it is the first of them. x_vec, s_vec: 16-byte (32 for FP32) rows of x, aligned chunks of scales.
-template <typename T, typename TS, int GROUP, int MT, int RT>
-__global__ void __launch_bounds__(32 * kGemvWarps)
-    gemv_int4_kernel(const Int4Params p, int rows, const T* __restrict__ x, long long ldx, const int* __restrict__ ids,
-                     T* __restrict__ y, long long ldy, bool x_vec, bool s_vec) {
-    using Math = Int4Math<T>;
-    constexpr int kOut = 16 * MT, kCols = 8 * RT, kPad = kOut + 1;
-    __shared__ float sums[kGemvWarps][kCols][kPad];
-    __shared__ unsigned char list[MFB_INT4_GEMV_ROWS];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = lane % 4;
-    const int i0 = blockIdx.x * kOut, n_left = p.n - i0;
-    int count = rows, expert = 0;
-    if (ids) {
-        const int mine = blockIdx.y;
-        const int a = lane < rows ? ids[lane] : -1, b = lane + 32 < rows ? ids[lane + 32] : -1;
-        expert = ids[mine];
-        if (expert < 0 || expert >= p.experts) {
-            if (expert >= p.experts && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(&g_status, kStatusBadIndex);
-            if (threadIdx.x < kOut && threadIdx.x < n_left) y[mine * ldy + i0 + threadIdx.x] = from_f32<T>(0.0f);
-            return;
-        }
-        const unsigned low = __ballot_sync(~0u, a == expert), high = __ballot_sync(~0u, b == expert);
-        const unsigned long long same = static_cast<unsigned long long>(high) << 32 | low;
-        if (__ffsll(static_cast<long long>(same)) - 1 != mine) return;
-        count = __popcll(same);
-        if (warp == 0) {
-            const unsigned below = (1u << lane) - 1;
-            if (a == expert) list[__popc(low & below)] = static_cast<unsigned char>(lane);
-            if (b == expert) list[__popc(low) + __popc(high & below)] = static_cast<unsigned char>(lane + 32);
-        }
-        __syncthreads();
+// The rows of x by expert: segment d holds rows order[begin[d]] .. order[begin[d + 1] - 1] of x.
+struct GemvSegments {
+    int count;
+    int expert[MFB_INT4_GEMV_ROWS];
+    int begin[MFB_INT4_GEMV_ROWS + 1];
+    int order[MFB_INT4_GEMV_ROWS];
+};
+
+// By one warp. Rows of no expert are in no segment.
+__device__ __forceinline__ void gemv_segments(const Int4Params& p, const int* ids, int rows, int lane, GemvSegments& g) {
+    if (!ids) {
+        if (lane == 0) g.count = 1, g.expert[0] = 0, g.begin[0] = 0, g.begin[1] = rows;
+        for (int r = lane; r < rows; r += 32) g.order[r] = r;
+        return;
     }
-    const long long row0 = static_cast<long long>(expert) * p.n + i0;
-    const int chunks = (p.k + 127) / 128;
-    for (int first = 0; first < count; first += kCols) {
-        const T* xr[RT];  // the row of x in this lane's column of B
-        bool live[RT];
+    int id[2];
+    unsigned long long same[2] = {0, 0};  // the rows of this row's expert
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int c = first + 8 * r + lane / 4;
-            live[r] = c < count;
-            xr[r] = x + (live[r] ? (ids ? list[c] : c) : 0) * ldx;
+    for (int h = 0; h < 2; ++h) {
+        const int r = lane + 32 * h;
+        id[h] = r < rows ? ids[r] : -1;
+        if (id[h] >= p.experts) {
+            if (blockIdx.x == 0) atomicOr(&g_status, kStatusBadIndex);
+            id[h] = -1;
         }
-        float acc[MT][RT][4] = {};
-        Int4Chunk<TS, GROUP, MT> next;
-        if (warp < chunks) next.load(p, row0, n_left, warp, lane, s_vec);
-        for (int chunk = warp; chunk < chunks; chunk += kGemvWarps) {
-            Int4Chunk<TS, GROUP, MT> cur = next;
-            if (chunk + kGemvWarps < chunks) next.load(p, row0, n_left, chunk + kGemvWarps, lane, s_vec);
-            uint32_t w[MT][2][4];
+    }
+    const unsigned low = __match_any_sync(~0u, id[0]), high = __match_any_sync(~0u, id[1]);
+    same[0] = low;
+    same[1] = static_cast<unsigned long long>(high) << 32;
+    if (rows > 32)
+        for (int l = 0; l < 32; ++l) {
+            if (__shfl_sync(~0u, id[1], l) == id[0]) same[0] |= 1ull << (32 + l);
+            if (__shfl_sync(~0u, id[0], l) == id[1]) same[1] |= 1ull << l;
+        }
+    int segments = 0, begin = 0;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+    for (int h = 0; h < 2; ++h) {
+        if (h == 1 && rows <= 32) break;
+        const int r = lane + 32 * h;
+        const bool first = id[h] >= 0 && __ffsll(static_cast<long long>(same[h])) - 1 == r;
+        const unsigned firsts = __ballot_sync(~0u, first);
+        const int d = segments + __popc(firsts & ((1u << lane) - 1));
+        int sum = first ? __popcll(same[h]) : 0;
+        const int mine = sum;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    w[mt][h][0] = cur.w[mt][h].x, w[mt][h][1] = cur.w[mt][h].y;
-                    w[mt][h][2] = cur.w[mt][h].z, w[mt][h][3] = cur.w[mt][h].w;
-                    regroup<GROUP>(w[mt][h], t);
-                }
-            float part[MT][RT][4];
+        for (int s = 1; s < 32; s *= 2) {
+            const int o = __shfl_up_sync(~0u, sum, s);
+            if (lane >= s) sum += o;
+        }
+        if (first) {
+            g.expert[d] = id[h];
+            int at = begin + sum - mine;
+            g.begin[d] = at;
+            for (unsigned long long m = same[h]; m; m &= m - 1) g.order[at++] = __ffsll(static_cast<long long>(m)) - 1;
+        }
+        segments += __popc(firsts);
+        begin += __shfl_sync(~0u, sum, 31);
+    }
+    if (lane == 0) g.count = segments, g.begin[segments] = begin;
+}
+
+// x_vec: 16-byte aligned rows of x; s_vec: aligned chunks of scales; kw_log: log2 of the warps along k.
+template <typename T, typename TS, int GROUP, int RT>
+__global__ void __launch_bounds__(32 * kGemvWarps, 1)
+    gemv_int4_kernel(const Int4Params p, int rows, const T* __restrict__ x, long long ldx, const int* __restrict__ ids,
+                     T* __restrict__ y, long long ldy, bool x_vec, bool s_vec, int kw_log) {
+    using Math = Int4Math<T>;
+    using Item = Int4Item<TS, GROUP>;
+    constexpr int kTerms = Math::kTerms, kCols = 8 * RT;
+    // Items in flight per warp, within 128 registers beside 16 * kTerms * RT of x.
+    constexpr int kItemRegs = 10 + 2 * (128 / GROUP * static_cast<int>(sizeof(TS)) + 3) / 4;
+    constexpr int kRoom = (88 - 16 * kTerms * RT) / kItemRegs;
+    constexpr int kDepth = kRoom > 4 ? 4 : kRoom < 2 ? 2 : kRoom;
+    extern __shared__ float4 sums[];  // [tile][kw][RT][lane]
+    __shared__ GemvSegments seg;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = lane % 4;
+    if (warp == 0) gemv_segments(p, ids, rows, lane, seg);
+    __syncthreads();
+
+    const int kw_count = 1 << kw_log, kw = warp & (kw_count - 1), tw = warp >> kw_log, tw_count = kGemvWarps >> kw_log;
+    const int chunks = (p.k + 127) / 128, tiles = (p.n + 15) / 16;
+    const int most = kGemvSlots / RT >> kw_log;
+    const long long all = static_cast<long long>(seg.count) * tiles;
+    long long from = all * blockIdx.x / gridDim.x;
+    const long long to = all * (blockIdx.x + 1) / gridDim.x;
+    while (from < to) {
+        const int d = static_cast<int>(from / tiles), m0 = static_cast<int>(from - static_cast<long long>(d) * tiles);
+        const int count = static_cast<int>(min(min(to - from, static_cast<long long>(tiles - m0)), static_cast<long long>(most)));
+        from += count;
+        const long long row0 = static_cast<long long>(seg.expert[d]) * p.n;
+        const int x_first = seg.begin[d], x_count = seg.begin[d + 1] - x_first;
+        for (int c0 = 0; c0 < x_count; c0 += kCols) {
+            const T* xr[RT];  // the row of x in this lane's column of B
+            bool live[RT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                constexpr int kSlots = GROUP / 32;  // word slots of a group
-                if (i % kSlots == 0)
+            for (int r = 0; r < RT; ++r) {
+                const int c = c0 + 8 * r + lane / 4;
+                live[r] = c < x_count;
+                xr[r] = x + (live[r] ? seg.order[x_first + c] : 0) * ldx;
+            }
+            uint32_t xb[RT][kTerms][4][4];  // [slot][b0, b1 of step 0, b0, b1 of step 1]
+            Item ring[kDepth];
+            int load_chunk = kw, load_tile = tw;
+            auto load = [&](Item& item) {
+                if (load_chunk >= chunks || tw >= count) return;
+                const int i = (m0 + load_tile) * 16;
+                item.load(p, row0 + i, p.n - i, load_chunk, lane, s_vec);
+                load_tile += tw_count;
+                if (load_tile >= count) load_tile = tw, load_chunk += kw_count;
+            };
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+            for (int i = 0; i < kDepth; ++i) load(ring[i]);
+            int chunk = kw, tile = tw;
+            while (chunk < chunks && tile < count) {
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
+                for (int at = 0; at < kDepth; ++at) {
+                    if (chunk >= chunks) continue;
+                    if (tile == tw) {  // a new chunk: lay out its columns of x
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) part[mt][r][e] = 0.0f;
-                uint32_t xv[RT][Math::kTerms][4];
-                const int j = chunk * 128 + slot_column<GROUP>(t, i);
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    if (live[r]) {
-                        load_x8<T>(xr[r], j, p.k, x_vec, xv[r]);
-                    } else {
+                            for (int r = 0; r < RT; ++r) {
+                                uint32_t v[kTerms][4] = {};
+                                if (live[r]) load_x8<T>(xr[r], chunk * 128 + slot_column<GROUP>(t, i), p.k, x_vec, v);
 #pragma unroll
-                        for (int u = 0; u < Math::kTerms; ++u)
+                                for (int u = 0; u < kTerms; ++u)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) xv[r][u][e] = 0;
+                                    for (int step = 0; step < 2; ++step) {
+                                        xb[r][u][i][2 * step] = __byte_perm(v[u][step], v[u][step + 2], 0x5410);
+                                        xb[r][u][i][2 * step + 1] = __byte_perm(v[u][step], v[u][step + 2], 0x7632);
+                                    }
+                            }
                     }
-                }
+                    const Item item = ring[at];
+                    load(ring[at]);
+                    uint32_t w[2][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    uint32_t lo[4], hi[4];  // rows g and g + 8, codes (i, i + 4)
-                    const int group = i / kSlots;
-                    Math::weights(w[mt][0][i], (cur.z[mt][0] >> (8 * group)) & 15u, lo);
-                    Math::weights(w[mt][1][i], (cur.z[mt][1] >> (8 * group)) & 15u, hi);
-#pragma unroll
-                    for (int step = 0; step < 2; ++step) {
-                        const uint32_t a[4] = {lo[2 * step], hi[2 * step], lo[2 * step + 1], hi[2 * step + 1]};
-#pragma unroll
-                        for (int r = 0; r < RT; ++r)
-#pragma unroll
-                            for (int u = Math::kTerms - 1; u >= 0; --u)
-                                Math::mma(part[mt][r], a, __byte_perm(xv[r][u][step], xv[r][u][step + 2], 0x5410),
-                                          __byte_perm(xv[r][u][step], xv[r][u][step + 2], 0x7632));
+                    for (int h = 0; h < 2; ++h) {
+                        w[h][0] = item.w[h].x, w[h][1] = item.w[h].y, w[h][2] = item.w[h].z, w[h][3] = item.w[h].w;
+                        regroup<GROUP>(w[h], t);
                     }
-                    if (i % kSlots == kSlots - 1) {
-                        const float s0 = to_f32(cur.s[mt][0][group]), s1 = to_f32(cur.s[mt][1][group]);
+                    float acc[RT][4] = {}, part[RT][4];
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
+                    for (int i = 0; i < 4; ++i) {
+                        constexpr int kSlots = GROUP / 32;  // word slots of a group
+                        const int group = i / kSlots;
+                        if (i % kSlots == 0)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[mt][r][e] = fmaf(e < 2 ? s0 : s1, part[mt][r][e], acc[mt][r][e]);
+                            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) part[r][e] = 0.0f;
+                        uint32_t lo[4], hi[4];  // rows g and g + 8, codes (i, i + 4)
+                        Math::weights(w[0][i], (item.z[0] >> (8 * group)) & 15u, lo);
+                        Math::weights(w[1][i], (item.z[1] >> (8 * group)) & 15u, hi);
+#pragma unroll
+                        for (int step = 0; step < 2; ++step) {
+                            const uint32_t a[4] = {lo[2 * step], hi[2 * step], lo[2 * step + 1], hi[2 * step + 1]};
+#pragma unroll
+                            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                for (int u = kTerms - 1; u >= 0; --u)
+                                    Math::mma(part[r], a, xb[r][u][i][2 * step], xb[r][u][i][2 * step + 1]);
+                        }
+                        if (i % kSlots == kSlots - 1) {
+                            const float s0 = to_f32(item.s[0][group]), s1 = to_f32(item.s[1][group]);
+#pragma unroll
+                            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(e < 2 ? s0 : s1, part[r][e], acc[r][e]);
+                        }
                     }
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        float4& slot = sums[(((tile << kw_log) + kw) * RT + r) * 32 + lane];
+                        float4 v = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+                        if (chunk != kw) {
+                            const float4 o = slot;
+                            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                        }
+                        slot = v;
+                    }
+                    tile += tw_count;
+                    if (tile >= count) tile = tw, chunk += kw_count;
                 }
             }
-        }
-        if (first > 0) __syncthreads();  // the sums of the rows before have been read
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sums[warp][8 * r + 2 * t + (e & 1)][16 * mt + lane / 4 + 8 * (e >> 1)] = acc[mt][r][e];
-        __syncthreads();
-        for (int at = threadIdx.x; at < kOut * kCols; at += 32 * kGemvWarps) {
-            const int c = at / kOut, i = at % kOut;
-            if (first + c >= count || i >= n_left) continue;
-            float sum = 0.0f;
-#pragma unroll
-            for (int v = 0; v < kGemvWarps; ++v) sum += sums[v][c][i];
-            y[(ids ? list[first + c] : first + c) * ldy + i0 + i] = from_f32<T>(sum);
+            __syncthreads();
+            const int split = min(kw_count, chunks);
+            for (int at = threadIdx.x; at < count * 16 * kCols; at += 32 * kGemvWarps) {
+                const int i = at & 15, rest = at >> 4;  // consecutive threads: consecutive outputs
+                const int c = rest % kCols, m = rest / kCols;
+                const int out = (m0 + m) * 16 + i;
+                if (c0 + c >= x_count || out >= p.n) continue;
+                const float* v = reinterpret_cast<const float*>(sums + ((m << kw_log) * RT + c / 8) * 32) +
+                                 ((i & 7) * 4 + c % 8 / 2) * 4 + (i >> 3) * 2 + (c & 1);
+                float sum = 0.0f;
+                for (int s = 0; s < split; ++s) sum += v[s * RT * 128];
+                y[seg.order[x_first + c0 + c] * ldy + out] = from_f32<T>(sum);
+            }
+            __syncthreads();
         }
     }
+    if (ids)  // rows of no expert
+        for (int r = 0; r < rows; ++r) {
+            const int e = ids[r];
+            if (e >= 0 && e < p.experts) continue;
+            for (int i = blockIdx.x * 32 * kGemvWarps + threadIdx.x; i < p.n; i += gridDim.x * 32 * kGemvWarps)
+                y[r * ldy + i] = from_f32<T>(0.0f);
+        }
 }
 
 template <typename T, typename TS, int GROUP>
-mfb_status_t gemv_int4_launch(const Int4Params& p, cudaStream_t stream, int rows, const T* x, long long ldx, const int* ids,
-                              T* y, long long ldy) {
-    constexpr int kVec = 8 * sizeof(T) < 16 ? 8 * sizeof(T) : 16;
-    const bool x_vec = (reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * sizeof(T))) % kVec == 0;
+mfb_status_t gemv_int4_launch(const Int4Params& p, int device, cudaStream_t stream, int rows, const T* x, long long ldx,
+                              const int* ids, T* y, long long ldy) {
+    const bool x_vec = (reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * sizeof(T))) % 16 == 0;
     constexpr int kGroups = 128 / GROUP;
     const bool s_vec = p.groups % kGroups == 0 && reinterpret_cast<uintptr_t>(p.scales) % (sizeof(TS) * kGroups) == 0 &&
                        reinterpret_cast<uintptr_t>(p.zeros) % kGroups == 0;
-    auto go = [&](auto mt, auto rt) {
-        constexpr int MT = decltype(mt)::value, RT = decltype(rt)::value;
-        const dim3 grid(static_cast<unsigned>((p.n + 16 * MT - 1) / (16 * MT)), ids ? static_cast<unsigned>(rows) : 1u);
-        gemv_int4_kernel<T, TS, GROUP, MT, RT><<<grid, 32 * kGemvWarps, 0, stream>>>(p, rows, x, ldx, ids, y, ldy, x_vec, s_vec);
+    const int chunks = (p.k + 127) / 128;
+    int kw_log = 0;
+    while (kw_log < 4 && (1 << kw_log) < chunks) ++kw_log;
+    const long long tiles = static_cast<long long>(ids ? rows : 1) * ((p.n + 15) / 16);
+    const unsigned grid = static_cast<unsigned>(std::min<long long>(tiles, sm_count(device)));
+    auto go = [&](auto rt) -> mfb_status_t {
+        const auto kernel = &gemv_int4_kernel<T, TS, GROUP, decltype(rt)::value>;
+        static std::atomic<unsigned long long> raised{0};  // devices whose shared-memory limit is raised
+        const unsigned long long bit = 1ull << (device & 63);
+        if (!(raised.load(std::memory_order_acquire) & bit)) {
+            MFB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemvSmem),
+                         "cudaFuncSetAttribute(gemv_int4)");
+            raised.fetch_or(bit, std::memory_order_release);
+        }
+        kernel<<<grid, 32 * kGemvWarps, kGemvSmem, stream>>>(p, rows, x, ldx, ids, y, ldy, x_vec, s_vec, kw_log);
+        MFB_CUDA_TRY(cudaGetLastError(), "gemv_int4 launch");
+        return MFB_OK;
     };
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
-    if (rows <= 8) {
-        if (p.n >= 32 * 148) go(Two{}, One{});
-        else go(One{}, One{});
-    } else {
-        if (p.n >= 32 * 148) go(Two{}, Two{});
-        else go(One{}, Two{});
-    }
-    MFB_CUDA_TRY(cudaGetLastError(), "gemv_int4 launch");
-    return MFB_OK;
+    // Two column tiles of x keep 16 rows in one pass over the codes; FP32 rows have no registers for that.
+    if constexpr (sizeof(T) == 2)
+        if (rows > 8 && !ids) return go(std::integral_constant<int, 2>());
+    return go(std::integral_constant<int, 1>());
 }
 
 mfb_status_t validate_int4(const mfb_int4_matrix* m, Int4Params* p) {
@@ -599,7 +692,7 @@ MFB_API mfb_status_t mfb_gemv_int4(int device, mfb_stream_t stream, const mfb_in
             const auto launch = m->group == 32   ? &gemv_int4_launch<T, TS, 32>
                                 : m->group == 64 ? &gemv_int4_launch<T, TS, 64>
                                                  : &gemv_int4_launch<T, TS, 128>;
-            return launch(p, reinterpret_cast<cudaStream_t>(stream), rows, static_cast<const T*>(x), ldx, expert_ids,
+            return launch(p, device, reinterpret_cast<cudaStream_t>(stream), rows, static_cast<const T*>(x), ldx, expert_ids,
                           static_cast<T*>(y), ldy);
         });
     });

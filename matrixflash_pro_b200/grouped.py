@@ -25,28 +25,32 @@ The work goes to `stream`, by default the current stream of the operands' device
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .errors import InvalidArgumentError, ShapeMismatchError
-from .gemm import GemmPrecision, checked_dim
+from .gemm import INT32_MAX, GemmPrecision
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MAX_GROUPS = 1024
 
 
+# The handle of a device's current stream as an int. torch.cuda.current_stream builds a Stream object, 2 us of a
+# call that takes 10 us of host time in all.
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream_of(device: torch.device, stream) -> int:
-    return int((stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream)
+    return _current_raw_stream(device.index) if stream is None else stream.cuda_stream
 
 
-def _new(shape, dtype, device, stream):
-    """An output that belongs to the stream that writes it."""
+def _new(like: torch.Tensor, shape, dtype, stream):
+    """An output on `like`'s device that belongs to the stream that writes it."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _rows_ld(t: torch.Tensor, what: str, dtype) -> int:
@@ -57,13 +61,13 @@ def _rows_ld(t: torch.Tensor, what: str, dtype) -> int:
         raise InvalidArgumentError(f"{what} must be {dtype}")
     rows, cols = t.shape
     ld, unit = t.stride()
-    if cols > 1 and unit != 1 and rows > 0:
+    if unit != 1 and cols > 1 and rows > 0:
         raise InvalidArgumentError(f"{what} must have unit column stride")
     if rows <= 1:
-        return max(cols, 1)
+        return cols or 1
     if ld < cols:
         raise InvalidArgumentError(f"{what} has rows that overlap")
-    return checked_dim(max(ld, 1))
+    return ld or 1
 
 
 def _stack_ld(t: torch.Tensor, what: str, dtype, shared_ok: bool):
@@ -73,22 +77,23 @@ def _stack_ld(t: torch.Tensor, what: str, dtype, shared_ok: bool):
     if t.dtype != dtype:
         raise InvalidArgumentError(f"{what} must be {dtype}")
     count, rows, cols = t.shape
-    if t.numel() == 0:
-        return max(cols, 1), rows * cols
     stride, ld, unit = t.stride()
-    if cols > 1 and unit != 1:
+    if not (count and rows and cols):
+        return cols or 1, rows * cols
+    if unit != 1 and cols > 1:
         raise InvalidArgumentError(f"{what} must have unit stride in its last dimension")
-    ld = cols if rows <= 1 else ld
-    if ld < cols:
+    if rows <= 1:
+        ld = cols
+    elif ld < cols:
         raise InvalidArgumentError(f"{what} has rows that overlap")
     if count <= 1:
         stride = 0 if shared_ok else rows * ld
     elif not shared_ok and stride < (rows - 1) * ld + cols:
         raise InvalidArgumentError(f"{what} has matrices that overlap")
-    return checked_dim(max(ld, 1)), stride
+    return ld, stride
 
 
-def _check(groups: int, offsets: torch.Tensor, tensors) -> None:
+def _check(groups: int, offsets: torch.Tensor, *tensors) -> None:
     """What both entry points ask of offsets and devices."""
     if groups > _MAX_GROUPS:
         raise InvalidArgumentError(f"at most {_MAX_GROUPS} groups are supported")
@@ -96,12 +101,12 @@ def _check(groups: int, offsets: torch.Tensor, tensors) -> None:
         raise InvalidArgumentError("offsets must be a contiguous int32 tensor")
     if offsets.dim() != 1 or offsets.shape[0] != groups + 1:
         raise ShapeMismatchError("offsets must have one entry more than there are groups")
+    if not offsets.is_cuda:
+        raise InvalidArgumentError("grouped products take CUDA tensors")
     device = offsets.device
     for t in tensors:
-        if not t.is_cuda:
-            raise InvalidArgumentError("grouped products take CUDA tensors")
-        if t.device != device:
-            raise InvalidArgumentError("operands of a grouped product must share one device")
+        if t is not None and t.device != device:
+            raise InvalidArgumentError("operands of a grouped product must share one CUDA device")
 
 
 def _dtype_of(t: torch.Tensor) -> int:
@@ -118,30 +123,44 @@ def _out_dtype(out: torch.Tensor, code: int) -> int:
     return got
 
 
+def _precision(precision) -> int:
+    return 0 if precision is GemmPrecision.fp32 else int(GemmPrecision(precision))
+
+
+def _launch(entry: str, what: str, device, stream, desc, offsets, a, b, out) -> None:
+    status = getattr(_lib.lib(), entry)(device.index, _stream_of(device, stream), desc, offsets.data_ptr(),
+                                        a.data_ptr(), b.data_ptr(), out.data_ptr())
+    if status:
+        _lib.check(status, what)
+
+
+def _desc(*fields):
+    """The descriptor; every dimension and row stride has to fit 32 bits."""
+    if max(fields[:7]) > INT32_MAX:
+        raise InvalidArgumentError("grouped product dimension exceeds the 32-bit limit")
+    return _lib.GroupedDesc(*fields)
+
+
 def _rows_times_stack(left, right, offsets, transpose, precision, out, stream, what):
+    dtype = left.dtype
     code = _dtype_of(left)
-    lda = _rows_ld(left, "left" if what == "grouped_matmul" else "grad", left.dtype)
-    ldb, stride = _stack_ld(right, "right", left.dtype, True)
+    lda = _rows_ld(left, "left" if what == "grouped_matmul" else "grad", dtype)
+    ldb, stride = _stack_ld(right, "right", dtype, True)
     groups, k, n = right.shape
     if transpose:
         k, n = n, k
-    rows = left.shape[0]
-    if left.shape[1] != k:
+    rows, cols = left.shape
+    if cols != k:
         raise ShapeMismatchError(f"{what} shape mismatch")
-    _check(groups, offsets, (left, right, offsets) if out is None else (left, right, offsets, out))
-    zero_rest = out is None
+    _check(groups, offsets, left, right, out)
     if out is None:
-        out = _new((rows, n), left.dtype, left.device, stream)
-        out_code, ldc = code, max(n, 1)
+        out, out_code, ldc, rest = _new(left, (rows, n), dtype, stream), code, n or 1, 1
     else:
         if tuple(out.shape) != (rows, n):
             raise ShapeMismatchError(f"{what} output shape mismatch")
-        out_code, ldc = _out_dtype(out, code), _rows_ld(out, "out", out.dtype)
-    desc = _lib.GroupedDesc(groups, checked_dim(rows), checked_dim(n), checked_dim(k), lda, ldb, ldc, stride, code,
-                            out_code, int(GemmPrecision(precision)), int(transpose), int(zero_rest))
-    _lib.check(_lib.lib().mfb_grouped_gemm(left.device.index, _stream_of(left.device, stream), ctypes.byref(desc),
-                                           offsets.data_ptr(), left.data_ptr(), right.data_ptr(), out.data_ptr()),
-               what)
+        out_code, ldc, rest = _out_dtype(out, code), _rows_ld(out, "out", out.dtype), 0
+    desc = _desc(groups, rows, n, k, lda, ldb, ldc, stride, code, out_code, _precision(precision), int(transpose), rest)
+    _launch("mfb_grouped_gemm", what, left.device, stream, desc, offsets, left, right, out)
     return out
 
 
@@ -176,18 +195,14 @@ def grouped_matmul_backward_right(grad: torch.Tensor, left: torch.Tensor, offset
     if offsets.dim() != 1 or offsets.shape[0] < 1:
         raise ShapeMismatchError("offsets must have one entry more than there are groups")
     groups = offsets.shape[0] - 1
-    _check(groups, offsets, (a, b, offsets) if out is None else (a, b, offsets, out))
+    _check(groups, offsets, a, b, out)
     if out is None:
-        out = _new((groups, k, n), grad.dtype, grad.device, stream)
-        out_code, ldc, stride = code, max(n, 1), k * n
+        out, out_code, ldc, stride = _new(grad, (groups, k, n), grad.dtype, stream), code, n or 1, k * n
     else:
         if tuple(out.shape) != (groups, k, n):
             raise ShapeMismatchError(f"{what} output shape mismatch")
         out_code = _out_dtype(out, code)
         ldc, stride = _stack_ld(out, "out", out.dtype, False)
-    desc = _lib.GroupedDesc(groups, checked_dim(rows), checked_dim(n), checked_dim(k), lda, ldb, ldc, stride, code,
-                            out_code, int(GemmPrecision(precision)), 0, 0)
-    _lib.check(_lib.lib().mfb_grouped_gemm_bwd_right(grad.device.index, _stream_of(grad.device, stream),
-                                                     ctypes.byref(desc), offsets.data_ptr(), a.data_ptr(),
-                                                     b.data_ptr(), out.data_ptr()), what)
+    desc = _desc(groups, rows, n, k, lda, ldb, ldc, stride, code, out_code, _precision(precision), 0, 0)
+    _launch("mfb_grouped_gemm_bwd_right", what, grad.device, stream, desc, offsets, a, b, out)
     return out

@@ -96,9 +96,9 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, symmetric: bool = Fals
         raise InvalidArgumentError("scales must be float32, float16 or bfloat16")
     *stack, n, k = weight.shape
     groups = -(-checked_dim(k) // group)
-    packed = _new((*stack, n, 16 * (-(-k // 32))), torch.uint8, weight.device, stream)
-    scales = _new((*stack, n, groups), scale_dtype, weight.device, stream)
-    zeros = None if symmetric else _new((*stack, n, groups), torch.uint8, weight.device, stream)
+    packed = _new(weight, (*stack, n, 16 * (-(-k // 32))), torch.uint8, stream)
+    scales = _new(weight, (*stack, n, groups), scale_dtype, stream)
+    zeros = None if symmetric else _new(weight, (*stack, n, groups), torch.uint8, stream)
     matrix = Int4Matrix(packed, scales, zeros, k, group)
     _lib.check(_lib.lib().mfb_quantize_int4(weight.device.index, _stream_of(weight.device, stream), weight.data_ptr(),
                                             DTYPES[weight.dtype], weight.stride(-2),
@@ -113,7 +113,7 @@ def dequantize_int4(matrix: Int4Matrix, dtype: torch.dtype | None = None, out: t
         dtype = matrix.scales.dtype if dtype is None else dtype
         if dtype not in DTYPES:
             raise InvalidArgumentError("dequantize_int4 gives float32, float16 or bfloat16")
-        out = _new(matrix.shape, dtype, matrix.device, stream)
+        out = _new(matrix.packed, matrix.shape, dtype, stream)
     else:
         if out.dtype not in DTYPES or (dtype is not None and dtype != out.dtype):
             raise InvalidArgumentError("out must have the asked type: float32, float16 or bfloat16")
@@ -138,18 +138,19 @@ def gemv_int4(matrix: Int4Matrix, x: torch.Tensor, out: torch.Tensor | None = No
     """y[r] = W x[r] for up to 64 rows of x [t,k] (float32, float16 or bfloat16); out [t,n] has x's type. A stack
     needs `experts`, a contiguous int32 CUDA tensor [t]: row r uses matrix experts[r]; a negative id gives a zero
     row, one past the stack a zero row and InvalidArgumentError from the next sync()."""
-    code = DTYPES.get(x.dtype)
+    dtype, device = x.dtype, matrix.device
+    code = DTYPES.get(dtype)
     if code is None:
         raise InvalidArgumentError("gemv_int4 takes float32, float16 or bfloat16 rows")
     if x.dim() != 2 or x.shape[1] != matrix.k:
         raise ShapeMismatchError("GEMV operand shape mismatch")
-    if x.device != matrix.device:
+    if x.device != device:
         raise InvalidArgumentError("x must be on the matrix's device")
-    rows, k = x.shape
+    rows = x.shape[0]
     if rows > GEMV_ROWS:
         raise InvalidArgumentError(f"gemv_int4 serves up to {GEMV_ROWS} rows (dequantize_int4 and a product serve more)")
     ldx, unit = x.stride()
-    if k > 1 and unit != 1 and rows:
+    if unit != 1 and matrix.k > 1 and rows:
         raise InvalidArgumentError("x must have unit column stride")
     ids = 0
     if experts is not None:
@@ -157,24 +158,26 @@ def gemv_int4(matrix: Int4Matrix, x: torch.Tensor, out: torch.Tensor | None = No
             raise InvalidArgumentError("experts must be a contiguous int32 tensor")
         if experts.shape[0] != rows:
             raise ShapeMismatchError("experts must have one entry per row")
-        if experts.device != matrix.device:
+        if experts.device != device:
             raise InvalidArgumentError("experts must be on the matrix's device")
         ids = experts.data_ptr()
     elif matrix.experts is not None:
         raise InvalidArgumentError("a stack of matrices needs an expert per row")
+    n = matrix.n
     if out is None:
-        out = _new((rows, matrix.n), x.dtype, x.device, stream)
-        ldy = matrix.n
+        out, ldy = _new(x, (rows, n), dtype, stream), n
     else:
-        if out.dtype != x.dtype or out.device != x.device:
+        if out.dtype != dtype or out.device != device:
             raise InvalidArgumentError("out must have x's type and device")
-        if tuple(out.shape) != (rows, matrix.n):
+        if tuple(out.shape) != (rows, n):
             raise ShapeMismatchError("GEMV operand shape mismatch")
         ldy, unit = out.stride()
-        if matrix.n > 1 and unit != 1 and rows:
+        if unit != 1 and n > 1 and rows:
             raise InvalidArgumentError("out must have unit column stride")
-        if rows > 1 and ldy < matrix.n:
+        if rows > 1 and ldy < n:
             raise InvalidArgumentError("out has rows that overlap")
-    _lib.check(_lib.lib().mfb_gemv_int4(matrix.device.index, _stream_of(matrix.device, stream), matrix._ref, rows,
-                                        x.data_ptr(), ldx, code, ids, out.data_ptr(), ldy), "gemv_int4")
+    status = _lib.lib().mfb_gemv_int4(device.index, _stream_of(device, stream), matrix._ref, rows, x.data_ptr(), ldx,
+                                      code, ids, out.data_ptr(), ldy)
+    if status:
+        _lib.check(status, "gemv_int4")
     return out
