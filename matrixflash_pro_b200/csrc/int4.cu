@@ -145,60 +145,56 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const Int4Params p
 // FP32 accumulator, its scale one FMA per accumulator. FP32 rows enter as three BF16 terms (exact), added into
 // the same accumulator, small ones first.
 //
-// Which columns meet in one MMA step is free as long as A and B agree, so a lane's word of eight codes serves two
-// steps as it lies: (word >> 4 i) & 0x000f000f holds codes i and i + 4. For groups of 64 and 32 the four lanes of
-// a row exchange words first, so that all columns of a step share one scale.
+// Which columns meet in one MMA step is free as long as A and B agree, so a word of eight codes serves two steps as
+// it lies: (word >> 4 i) & 0x000f000f holds codes i and i + 4. The four lanes of a row take four words of one group
+// at a time, so that all columns of a step share one scale.
 //
 // One block of 16 warps per SM takes an even share of the 16-row tiles. Its warps split the columns (KW warps,
 // every KW-th chunk each) and, where there are fewer chunks than warps, the tiles. A warp goes chunk by chunk
-// through the tiles, so a chunk of x is loaded and laid out once for all of them; codes and scales of the next
-// tiles are in flight in registers meanwhile. Sums wait in shared memory, a slot per tile, warp and lane, and are
-// added up in a fixed order at the end.
+// through the tiles, two side by side (two independent MMA chains), so a chunk of x is loaded and laid out once for
+// all of them. Codes come by TMA into a ring that belongs to the warp; the scales and zero points of a block's tiles
+// by one bulk copy (loads of a few bytes per row into registers cost as much time as all else together: 108 us
+// against 61 for 9 of 16 experts of 2048 x 16384). Sums wait in shared memory, a slot per tile, warp and lane, and
+// are added up in a fixed order.
 
-template <typename T>
-struct Int4Math {  // FP16
-    static constexpr int kTerms = 1;
-    __device__ __forceinline__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// Codes as 16-bit floats. The bits of a code in the low half of a 16-bit word are a subnormal number, q times the
+// type's smallest one (in bits 4-7: 16 times that; BF16's exponent field is still 0 or 1 there), and one FMA by a
+// power of two less z gives (q - z) * kUnit exactly. A word of eight codes costs one shift, four ANDs, four FMAs.
+struct Int4MathF16 {
+    static constexpr float kUnit = 0x1p-10f;
+    static constexpr uint32_t kLow = 0x74007400u, kHigh = 0x64006400u, kMinusLow = 0xf400f400u;  // 2^14, 2^10, -2^14
+    __device__ __forceinline__ static uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
     }
-    // Codes i and i + 4 of a word, less z, for i = 0..3: 1024 + q (or 1024 + 16 q) has q in its low bits.
-    __device__ __forceinline__ static void weights(uint32_t word, uint32_t z, uint32_t (&out)[4]) {
-        const float zf = static_cast<float>(z);
-        const __half2 low = __float2half2_rn(1024.0f + zf), high = __float2half2_rn(-64.0f - zf);
-        const __half2 sixteenth = __float2half2_rn(0.0625f);
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-            uint32_t u = ((word >> (4 * i)) & 0x00f000f0u) | 0x64006400u;
-            const __half2 d = __hsub2(reinterpret_cast<__half2&>(v), low);
-            const __half2 e = __hfma2(reinterpret_cast<__half2&>(u), sixteenth, high);
-            out[i] = reinterpret_cast<const uint32_t&>(d);
-            out[i + 1] = reinterpret_cast<const uint32_t&>(e);
-        }
+    __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                               const float (&c)[4]) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     }
 };
-
 struct Int4MathBf16 {
-    __device__ __forceinline__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    static constexpr float kUnit = 0x1p-6f;
+    static constexpr uint32_t kLow = 0x7f007f00u, kHigh = 0x7d007d00u, kMinusLow = 0xff00ff00u;  // 2^127, 2^123, -2^127
+    __device__ __forceinline__ static uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
     }
-    __device__ __forceinline__ static void weights(uint32_t word, uint32_t z, uint32_t (&out)[4]) {
-        const __nv_bfloat162 offset = __float2bfloat162_rn(128.0f + static_cast<float>(z));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;  // 128 + q
-            const __nv_bfloat162 d = __hsub2(reinterpret_cast<__nv_bfloat162&>(v), offset);
-            out[i] = reinterpret_cast<const uint32_t&>(d);
-        }
+    __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                               const float (&c)[4]) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     }
+};
+template <typename T>
+struct Int4Math : Int4MathF16 {
+    static constexpr int kTerms = 1;
 };
 template <>
 struct Int4Math<__nv_bfloat16> : Int4MathBf16 {
@@ -209,118 +205,122 @@ struct Int4Math<float> : Int4MathBf16 {
     static constexpr int kTerms = 3;
 };
 
-// Eight consecutive values of a row of x from column j on (0 behind column k), as 16-bit pairs per term.
-template <typename T>
-__device__ __forceinline__ void load_x8(const T* row, int j, int k, bool vec, uint32_t (&out)[Int4Math<T>::kTerms][4]) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec && j + 8 <= k) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + j));
-            out[0][0] = v.x, out[0][1] = v.y, out[0][2] = v.z, out[0][3] = v.w;
-            return;
-        }
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = j + 2 * i < k ? __ldg(h + j + 2 * i) : 0, hi = j + 2 * i + 1 < k ? __ldg(h + j + 2 * i + 1) : 0;
-            out[0][i] = lo | hi << 16;
-        }
-    } else {
-        float v[8];
-        if (vec && j + 8 <= k) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(row + j)), b = __ldg(reinterpret_cast<const float4*>(row + j) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = j + i < k ? __ldg(reinterpret_cast<const float*>(row) + j + i) : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float lo = v[2 * i], hi = v[2 * i + 1];
-            asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(out[0][i]) : "f"(hi), "f"(lo));
-#pragma unroll
-            for (int t = 1; t < 3; ++t) {
-                lo -= __uint_as_float(out[t - 1][i] << 16);
-                hi -= __uint_as_float(out[t - 1][i] & 0xffff0000u);
-                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(out[t][i]) : "f"(hi), "f"(lo));
-            }
-        }
-    }
+// -z * kUnit in both halves, z being byte `group` of zeros.
+template <typename Math>
+__device__ __forceinline__ uint32_t int4_zero(uint32_t zeros, int group) {
+    return Math::fma2(__byte_perm(zeros, 0, 0x4040 + 0x0101 * group), Math::kMinusLow, 0x80008000u);
+}
+// (q - z) * kUnit for codes i and i + 4 of a word, i = 0..3.
+template <typename Math>
+__device__ __forceinline__ void int4_weights(uint32_t word, uint32_t zero, uint32_t (&out)[4]) {
+    out[0] = Math::fma2(word & 0x000f000fu, Math::kLow, zero);
+    out[1] = Math::fma2(word & 0x00f000f0u, Math::kHigh, zero);
+    word >>= 8;
+    out[2] = Math::fma2(word & 0x000f000fu, Math::kLow, zero);
+    out[3] = Math::fma2(word & 0x00f000f0u, Math::kHigh, zero);
 }
 
-// Codes, scales and zero points of one tile and chunk: rows g and g + 8 of this lane.
-template <typename TS, int GROUP>
-struct Int4Item {
-    static constexpr int kGroups = 128 / GROUP;
-    uint4 w[2];
-    TS s[2][kGroups];
-    uint32_t z[2];  // one byte per group
+// Eight consecutive values of a row of x from column j on, 0 behind column k.
+template <typename T>
+struct GemvX8 {
+    uint32_t w[2 * sizeof(T)];
 
-    // vec: whole chunks of groups, aligned.
-    __device__ __forceinline__ void load(const Int4Params& p, long long row0, int n_left, int chunk, int lane, bool vec) {
-        const int byte = chunk * 64 + lane % 4 * 16;
+    __device__ __forceinline__ void load(const T* row, int j, int k, bool vec) {
+        if (vec && j + 8 <= k) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const long long row = row0 + min(h * 8 + lane / 4, n_left - 1);  // rows past the end repeat the last
-            w[h] = make_uint4(0, 0, 0, 0);
-            if (byte < p.row_bytes)
-                asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(w[h].x), "=r"(w[h].y), "=r"(w[h].z), "=r"(w[h].w)
-                             : "l"(p.packed + row * p.row_bytes + byte));
-            const long long at = row * p.groups + chunk * kGroups;
-            const TS* sp = static_cast<const TS*>(p.scales) + at;
-            z[h] = 0x08080808u;
-            if (vec) {
-                struct alignas(sizeof(TS) * kGroups) Vec {
-                    TS v[kGroups];
-                };
-                const Vec v = *reinterpret_cast<const Vec*>(sp);
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + j) + i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+        } else if constexpr (sizeof(T) == 2) {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(row) + j;
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) s[h][i] = v.v[i];
-                if (p.zeros) {
-                    if (kGroups == 4) z[h] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
-                    else if (kGroups == 2) z[h] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
-                    else z[h] = __ldg(p.zeros + at);
-                }
-            } else {
-                if (p.zeros) z[h] = 0;
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = j + 2 * i < k ? __ldg(h + 2 * i) : 0, hi = j + 2 * i + 1 < k ? __ldg(h + 2 * i + 1) : 0;
+                w[i] = lo | hi << 16;
+            }
+        } else {
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    const bool in = chunk * kGroups + i < p.groups;
-                    s[h][i] = in ? sp[i] : from_f32<TS>(0.0f);
-                    if (p.zeros && in) z[h] |= static_cast<uint32_t>(__ldg(p.zeros + at + i)) << (8 * i);
+            for (int i = 0; i < 8; ++i) w[i] = j + i < k ? __ldg(reinterpret_cast<const uint32_t*>(row) + j + i) : 0;
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) w[i] = 0;
+    }
+    // B registers of the two steps that a word of codes serves: values (0, 4), (1, 5) and (2, 6), (3, 7), per term.
+    template <int TERMS>
+    __device__ __forceinline__ void lay_out(uint32_t (&b)[TERMS][4]) const {
+        uint32_t v[TERMS][4];
+        if constexpr (TERMS == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[0][i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float lo = __uint_as_float(w[2 * i]), hi = __uint_as_float(w[2 * i + 1]);
+                asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v[0][i]) : "f"(hi), "f"(lo));
+#pragma unroll
+                for (int t = 1; t < TERMS; ++t) {
+                    lo -= __uint_as_float(v[t - 1][i] << 16);
+                    hi -= __uint_as_float(v[t - 1][i] & 0xffff0000u);
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[t][i]) : "f"(hi), "f"(lo));
                 }
             }
         }
+#pragma unroll
+        for (int u = 0; u < TERMS; ++u)
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+                b[u][2 * step] = __byte_perm(v[u][step], v[u][step + 2], 0x5410);
+                b[u][2 * step + 1] = __byte_perm(v[u][step], v[u][step + 2], 0x7632);
+            }
     }
 };
 
-// Exchanges words between the four lanes of a row so that word slots of one group hold codes of one group:
-// slot i of lane t then starts at column slot_column(t, i) of the chunk.
-template <int GROUP>
-__device__ __forceinline__ void regroup(uint32_t (&w)[4], int t) {
-    if (GROUP <= 64) {
-        const bool upper = t >= 2;
-        const uint32_t a = __shfl_xor_sync(~0u, upper ? w[0] : w[2], 2), b = __shfl_xor_sync(~0u, upper ? w[1] : w[3], 2);
-        if (upper) w[0] = a, w[1] = b;
-        else w[2] = a, w[3] = b;
-    }
-    if (GROUP == 32) {
-        const bool odd = t & 1;
-        const uint32_t a = __shfl_xor_sync(~0u, odd ? w[0] : w[1], 1), b = __shfl_xor_sync(~0u, odd ? w[2] : w[3], 1);
-        if (odd) w[0] = a, w[2] = b;
-        else w[1] = a, w[3] = b;
-    }
+// Scales (or zero points, a byte each) of one row and chunk.
+template <typename TS, int GROUPS>
+struct alignas(GROUPS * sizeof(TS)) GemvScales {
+    TS v[GROUPS];
+};
+
+// Copies `bytes` from global to shared memory, both 16-byte aligned: the whole 16 bytes by TMA onto `bar`, whose
+// expected bytes it returns, the last few by this thread.
+__device__ __forceinline__ uint32_t copy_bulk(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+    const uint32_t whole = bytes & ~15u;
+    for (uint32_t i = whole; i < bytes; ++i)
+        static_cast<unsigned char*>(to)[i] = static_cast<const unsigned char*>(from)[i];
+    if (whole)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)),
+                     "l"(from), "r"(whole), "r"(smem_u32(bar))
+                     : "memory");
+    return whole;
 }
+
+// Lane t's word i of the 64 bytes that 128 columns take: words of one group are GROUP / 32 slots in a row per lane.
 template <int GROUP>
-__device__ __forceinline__ int slot_column(int t, int i) {
-    if (GROUP == 128) return 32 * t + 8 * i;
-    if (GROUP == 64) return 32 * ((t & 1) + 2 * (i >> 1)) + 8 * ((i & 1) + 2 * (t >> 1));
-    return 32 * i + 8 * t;
+__device__ __forceinline__ int slot_word(int t, int i) {
+    constexpr int kSlots = GROUP / 32;
+    return i / kSlots * 4 * kSlots + t * kSlots + i % kSlots;
+}
+
+// Row of a tile (0..7, and 8 more) that lanes 4 g .. 4 g + 3 take. Any order would do; this one lets the lanes that
+// read shared memory together read different banks of the swizzled box.
+template <int GROUP, int HALVES>
+__device__ __forceinline__ int tile_row(int g) {
+    if (HALVES == 1 || GROUP == 32) return g;
+    return GROUP == 64 ? (g << 1 & 6) | g >> 2 : g >> 1 | (g & 1) << 2;
+}
+template <int GROUP, int HALVES>
+__device__ __forceinline__ int tile_lane(int row) {
+    if (HALVES == 1 || GROUP == 32) return row;
+    return GROUP == 64 ? row >> 1 | (row & 1) << 2 : (row << 1 & 6) | row >> 2;
 }
 
 constexpr int kGemvWarps = 16;
-constexpr int kGemvSlots = 128;  // 16-row tiles times warps along k whose sums one block holds at a time
-constexpr int kGemvSmem = kGemvSlots * 32 * 16;
+constexpr int kGemvDepth = 4;  // KB of codes in flight per warp: 64 KB per SM
+constexpr int kGemvRing = kGemvWarps * kGemvDepth * 1024;
+constexpr int kGemvSmem = 224 * 1024;  // the ring, then sums and scales of as many tiles as fit
 
 // The rows of x by expert: segment d holds rows order[begin[d]] .. order[begin[d + 1] - 1] of x.
 struct GemvSegments {
@@ -383,37 +383,80 @@ __device__ __forceinline__ void gemv_segments(const Int4Params& p, const int* id
     if (lane == 0) g.count = segments, g.begin[segments] = begin;
 }
 
-// x_vec: 16-byte aligned rows of x; s_vec: aligned chunks of scales; kw_log: log2 of the warps along k.
-template <typename T, typename TS, int GROUP, int RT>
+// x_vec: 16-byte aligned rows of x; s_bulk: scales and zero points of whole chunks that a bulk copy can take; kw_log:
+// log2 of the warps along k; most: tiles whose sums and scales shared memory holds.
+template <typename T, typename TS, int GROUP, int RT, int HALVES>
 __global__ void __launch_bounds__(32 * kGemvWarps, 1)
-    gemv_int4_kernel(const Int4Params p, int rows, const T* __restrict__ x, long long ldx, const int* __restrict__ ids,
-                     T* __restrict__ y, long long ldy, bool x_vec, bool s_vec, int kw_log) {
+    gemv_int4_kernel(const __grid_constant__ CUtensorMap codes, const Int4Params p, int rows, const T* __restrict__ x,
+                     long long ldx, const int* __restrict__ ids, T* __restrict__ y, long long ldy, bool x_vec, bool s_bulk,
+                     int kw_log, int most, uint64_t wait_limit_ns) {
     using Math = Int4Math<T>;
-    using Item = Int4Item<TS, GROUP>;
-    constexpr int kTerms = Math::kTerms, kCols = 8 * RT;
-    // Items in flight per warp, within 128 registers beside 16 * kTerms * RT of x.
-    constexpr int kItemRegs = 10 + 2 * (128 / GROUP * static_cast<int>(sizeof(TS)) + 3) / 4;
-    constexpr int kRoom = (88 - 16 * kTerms * RT) / kItemRegs;
-    constexpr int kDepth = kRoom > 4 ? 4 : kRoom < 2 ? 2 : kRoom;
-    extern __shared__ float4 sums[];  // [tile][kw][RT][lane]
+    constexpr int kTerms = Math::kTerms, kCols = 8 * RT, kChunk = 128 * HALVES, kGroups = kChunk / GROUP;
+    constexpr int kSlots = GROUP / 32, kDepth = kGemvDepth / HALVES;
+    extern __shared__ __align__(1024) uint4 ring[];                   // [warp][stage][16 rows][4 * HALVES pieces]
+    float4* sums = reinterpret_cast<float4*>(ring + kGemvRing / 16);  // [tile][kw][RT][lane]
     __shared__ GemvSegments seg;
+    __shared__ uint64_t bars[kGemvWarps][kDepth], scale_bar;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = lane % 4;
+    const int my_row = tile_row<GROUP, HALVES>(lane / 4);  // and 8 more
     if (warp == 0) gemv_segments(p, ids, rows, lane, seg);
+    if (lane < kDepth) {
+        mbar_init(&bars[warp][lane], 1);
+        if (threadIdx.x == 0) mbar_init(&scale_bar, 1);
+        fence_barrier_init();
+        fence_proxy_async_smem();
+    }
     __syncthreads();
 
     const int kw_count = 1 << kw_log, kw = warp & (kw_count - 1), tw = warp >> kw_log, tw_count = kGemvWarps >> kw_log;
-    const int chunks = (p.k + 127) / 128, tiles = (p.n + 15) / 16;
-    const int most = kGemvSlots / RT >> kw_log;
-    const long long all = static_cast<long long>(seg.count) * tiles;
-    long long from = all * blockIdx.x / gridDim.x;
-    const long long to = all * (blockIdx.x + 1) / gridDim.x;
-    while (from < to) {
-        const int d = static_cast<int>(from / tiles), m0 = static_cast<int>(from - static_cast<long long>(d) * tiles);
-        const int count = static_cast<int>(min(min(to - from, static_cast<long long>(tiles - m0)), static_cast<long long>(most)));
-        from += count;
+    const int chunks = (p.k + kChunk - 1) / kChunk, tiles = (p.n + 15) / 16;
+    uint4* my_ring = ring + warp * kGemvDepth * 64;
+    float4* my_sums = sums + ((tw << kw_log) + kw) * RT * 32 + lane;
+    TS* scales = reinterpret_cast<TS*>(sums + (most << kw_log) * RT * 32);                     // [tile][16 rows][group]
+    unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + most * 16 * p.groups);
+    const bool whole = p.groups % kGroups == 0;  // every chunk has all its groups, vectors are aligned
+    int load_stage = 0, stage = 0;
+    uint32_t parity = 0;  // of the barriers' round that `stage` is in
+    uint32_t scale_parity = 0;
+    bool ok = true;
+    // An even share of all tiles: segment d, tiles m0 .. of it, left of them in all.
+    const unsigned all = static_cast<unsigned>(seg.count) * tiles, share = all / gridDim.x, more = all % gridDim.x;
+    const unsigned from = blockIdx.x * share + min(blockIdx.x, more);
+    int left = static_cast<int>(share + (blockIdx.x < more ? 1 : 0));
+    int d = static_cast<int>(from / tiles), m0 = static_cast<int>(from - d * static_cast<unsigned>(tiles));
+    for (int count; ok && left > 0; left -= count, m0 += count) {
+        if (m0 == tiles) m0 = 0, ++d;
+        count = min(min(left, tiles - m0), most);
+        const int mine = (count - tw + tw_count - 1) / tw_count;  // tiles of this warp: tw, tw + tw_count, ..
         const long long row0 = static_cast<long long>(seg.expert[d]) * p.n;
         const int x_first = seg.begin[d], x_count = seg.begin[d + 1] - x_first;
+        const TS* s_matrix = static_cast<const TS*>(p.scales) + row0 * p.groups;
+        const unsigned char* z_matrix = p.zeros + row0 * p.groups;
+        if (s_bulk && threadIdx.x == 0) {
+            const long long first = static_cast<long long>(m0) * 16 * p.groups;
+            const uint32_t cells = static_cast<uint32_t>(min(count * 16, p.n - m0 * 16)) * p.groups;
+            uint32_t bytes = copy_bulk(scales, s_matrix + first, cells * static_cast<uint32_t>(sizeof(TS)), &scale_bar);
+            if (p.zeros) bytes += copy_bulk(zeros, z_matrix + first, cells, &scale_bar);
+            mbar_arrive_expect_tx(&scale_bar, bytes);
+        }
+        bool scales_here = !s_bulk;
         for (int c0 = 0; c0 < x_count; c0 += kCols) {
+            // Codes: this warp's tiles of chunk kw, then of chunk kw + kw_count, ..
+            int load_chunk = mine > 0 ? kw : chunks, load_tile = 0;
+            const int box_row = static_cast<int>(row0) + (m0 + tw) * 16;  // rows past the matrix: read, or 0, and not used
+            auto load = [&]() {
+                if (load_chunk >= chunks) return;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&bars[warp][load_stage], 1024 * HALVES);
+                    tma_load_2d(my_ring + load_stage * 64 * HALVES, &codes, &bars[warp][load_stage], load_chunk * 64 * HALVES,
+                                box_row + load_tile * tw_count * 16);
+                }
+                if (++load_tile == mine) load_tile = 0, load_chunk += kw_count;
+                if (++load_stage == kDepth) load_stage = 0;
+            };
+#pragma unroll 1
+            for (int i = 0; i < kDepth; ++i) load();
+
             const T* xr[RT];  // the row of x in this lane's column of B
             bool live[RT];
 #pragma unroll
@@ -422,92 +465,164 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
                 live[r] = c < x_count;
                 xr[r] = x + (live[r] ? seg.order[x_first + c] : 0) * ldx;
             }
-            uint32_t xb[RT][kTerms][4][4];  // [slot][b0, b1 of step 0, b0, b1 of step 1]
-            Item ring[kDepth];
-            int load_chunk = kw, load_tile = tw;
-            auto load = [&](Item& item) {
-                if (load_chunk >= chunks || tw >= count) return;
-                const int i = (m0 + load_tile) * 16;
-                item.load(p, row0 + i, p.n - i, load_chunk, lane, s_vec);
-                load_tile += tw_count;
-                if (load_tile >= count) load_tile = tw, load_chunk += kw_count;
+            // Scales and zero points (a byte per group) of row r of the tiles, groups of half b of a chunk.
+            using Scales = GemvScales<TS, 128 / GROUP>;
+            auto read_scales = [&](int r, int chunk, int b, Scales& s, uint32_t& z) {
+                constexpr int kHalf = 128 / GROUP;
+                const int g0 = chunk * kGroups + b * kHalf;
+                z = 0x08080808u;
+                if (s_bulk && whole) {
+                    s = *reinterpret_cast<const Scales*>(scales + r * p.groups + g0);
+                    if (p.zeros) {
+                        const unsigned char* at = zeros + r * p.groups + g0;
+                        if (kHalf == 4) z = *reinterpret_cast<const uint32_t*>(at);
+                        else if (kHalf == 2) z = *reinterpret_cast<const uint16_t*>(at);
+                        else z = *at;
+                    }
+                    return;
+                }
+                const long long at = static_cast<long long>(min(m0 * 16 + r, p.n - 1)) * p.groups;
+                const TS* sp = s_bulk ? scales + r * p.groups : s_matrix + at;
+                const unsigned char* zp = s_bulk ? zeros + r * p.groups : z_matrix + at;
+                if (p.zeros) z = 0;
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) {
+                    const bool in = g0 + i < p.groups;
+                    s.v[i] = in ? sp[g0 + i] : from_f32<TS>(0.0f);
+                    if (p.zeros && in) z |= static_cast<uint32_t>(zp[g0 + i]) << (8 * i);
+                }
             };
+
+            uint32_t xb[HALVES][RT][4][kTerms][4];
+            // N tiles from tile j on: independent chains of MMAs side by side.
+            auto step_over = [&](auto n_, int j, int chunk) {
+                constexpr int N = decltype(n_)::value;
+                const uint32_t* box[N];
 #pragma unroll
-            for (int i = 0; i < kDepth; ++i) load(ring[i]);
-            int chunk = kw, tile = tw;
-            while (chunk < chunks && tile < count) {
+                for (int u = 0; u < N; ++u) {
+                    ok = ok && mbar_wait_bounded(&bars[warp][stage], parity, wait_limit_ns, nullptr);
+                    box[u] = reinterpret_cast<const uint32_t*>(my_ring + stage * 64 * HALVES);
+                    if (++stage == kDepth) stage = 0, parity ^= 1;
+                }
+                float acc[N][RT][4];
 #pragma unroll
-                for (int at = 0; at < kDepth; ++at) {
-                    if (chunk >= chunks) continue;
-                    if (tile == tw) {  // a new chunk: lay out its columns of x
+                for (int b = 0; b < HALVES; ++b) {
+                    Scales s[N][2];
+                    uint32_t z[N][2], w[N][2][4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                    for (int u = 0; u < N; ++u)
 #pragma unroll
-                            for (int r = 0; r < RT; ++r) {
-                                uint32_t v[kTerms][4] = {};
-                                if (live[r]) load_x8<T>(xr[r], chunk * 128 + slot_column<GROUP>(t, i), p.k, x_vec, v);
+                        for (int h = 0; h < 2; ++h) {
+                            const int r = my_row + 8 * h;
+                            read_scales((tw + (j + u) * tw_count) * 16 + r, chunk, b, s[u][h], z[u][h]);
+                            // 16-byte pieces are swizzled by the row: all 8 pieces of 128 bytes, or 4 of 64
+                            const int swizzle = HALVES == 2 ? (r & 7) * 4 : (r >> 1 & 3) * 4;
 #pragma unroll
-                                for (int u = 0; u < kTerms; ++u)
-#pragma unroll
-                                    for (int step = 0; step < 2; ++step) {
-                                        xb[r][u][i][2 * step] = __byte_perm(v[u][step], v[u][step + 2], 0x5410);
-                                        xb[r][u][i][2 * step + 1] = __byte_perm(v[u][step], v[u][step + 2], 0x7632);
-                                    }
+                            for (int i = 0; i < 4; i += kSlots) {
+                                const uint32_t* from_w = box[u] + r * 16 * HALVES + ((b * 16 + slot_word<GROUP>(t, i)) ^ swizzle);
+                                if constexpr (kSlots == 4) {
+                                    const uint4 v = *reinterpret_cast<const uint4*>(from_w);
+                                    w[u][h][0] = v.x, w[u][h][1] = v.y, w[u][h][2] = v.z, w[u][h][3] = v.w;
+                                } else if constexpr (kSlots == 2) {
+                                    const uint2 v = *reinterpret_cast<const uint2*>(from_w);
+                                    w[u][h][i] = v.x, w[u][h][i + 1] = v.y;
+                                } else {
+                                    w[u][h][i] = *from_w;
+                                }
                             }
-                    }
-                    const Item item = ring[at];
-                    load(ring[at]);
-                    uint32_t w[2][4];
+                        }
+                    if (b == HALVES - 1) {
+                        __syncwarp();  // every lane has read the boxes
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        w[h][0] = item.w[h].x, w[h][1] = item.w[h].y, w[h][2] = item.w[h].z, w[h][3] = item.w[h].w;
-                        regroup<GROUP>(w[h], t);
+                        for (int u = 0; u < N; ++u) load();
                     }
-                    float acc[RT][4] = {}, part[RT][4];
+                    float part[N][RT][4];
+                    uint32_t zero[N][2];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        constexpr int kSlots = GROUP / 32;  // word slots of a group
                         const int group = i / kSlots;
-                        if (i % kSlots == 0)
 #pragma unroll
-                            for (int r = 0; r < RT; ++r)
+                        for (int u = 0; u < N; ++u) {
+                            uint32_t a[2][4];  // rows my_row + 8 h, codes (i, i + 4)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) part[r][e] = 0.0f;
-                        uint32_t lo[4], hi[4];  // rows g and g + 8, codes (i, i + 4)
-                        Math::weights(w[0][i], (item.z[0] >> (8 * group)) & 15u, lo);
-                        Math::weights(w[1][i], (item.z[1] >> (8 * group)) & 15u, hi);
+                            for (int h = 0; h < 2; ++h) {
+                                if (i % kSlots == 0) zero[u][h] = int4_zero<Math>(z[u][h], group);
+                                int4_weights<Math>(w[u][h][i], zero[u][h], a[h]);
+                            }
 #pragma unroll
-                        for (int step = 0; step < 2; ++step) {
-                            const uint32_t a[4] = {lo[2 * step], hi[2 * step], lo[2 * step + 1], hi[2 * step + 1]};
+                            for (int step = 0; step < 2; ++step) {
+                                const uint32_t av[4] = {a[0][2 * step], a[1][2 * step], a[0][2 * step + 1], a[1][2 * step + 1]};
 #pragma unroll
-                            for (int r = 0; r < RT; ++r)
+                                for (int r = 0; r < RT; ++r)
 #pragma unroll
-                                for (int u = kTerms - 1; u >= 0; --u)
-                                    Math::mma(part[r], a, xb[r][u][i][2 * step], xb[r][u][i][2 * step + 1]);
-                        }
-                        if (i % kSlots == kSlots - 1) {
-                            const float s0 = to_f32(item.s[0][group]), s1 = to_f32(item.s[1][group]);
+                                    for (int e = kTerms - 1; e >= 0; --e) {
+                                        const uint32_t(&xv)[4] = xb[b][r][i][e];
+                                        const float none[4] = {};
+                                        const bool first = i % kSlots == 0 && step == 0 && e == kTerms - 1;
+                                        if (first) Math::mma(part[u][r], av, xv[2 * step], xv[2 * step + 1], none);
+                                        else Math::mma(part[u][r], av, xv[2 * step], xv[2 * step + 1], part[u][r]);
+                                    }
+                            }
+                            if (i % kSlots == kSlots - 1) {
+                                const float s0 = to_f32(s[u][0].v[group]), s1 = to_f32(s[u][1].v[group]);
 #pragma unroll
-                            for (int r = 0; r < RT; ++r)
+                                for (int r = 0; r < RT; ++r)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(e < 2 ? s0 : s1, part[r][e], acc[r][e]);
+                                    for (int e = 0; e < 4; ++e)
+                                        acc[u][r][e] = b == 0 && i == kSlots - 1
+                                                           ? (e < 2 ? s0 : s1) * part[u][r][e]
+                                                           : fmaf(e < 2 ? s0 : s1, part[u][r][e], acc[u][r][e]);
+                            }
                         }
                     }
+                }
+#pragma unroll
+                for (int u = 0; u < N; ++u)
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
-                        float4& slot = sums[(((tile << kw_log) + kw) * RT + r) * 32 + lane];
-                        float4 v = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+                        // tile tw + (j + u) tw_count: kw_count slots a tile, kw_count tw_count = kGemvWarps
+                        float4& slot = my_sums[((j + u) * kGemvWarps * RT + r) * 32];
+                        float4 v = make_float4(acc[u][r][0], acc[u][r][1], acc[u][r][2], acc[u][r][3]);
                         if (chunk != kw) {
                             const float4 o = slot;
                             v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
                         }
                         slot = v;
                     }
-                    tile += tw_count;
-                    if (tile >= count) tile = tw, chunk += kw_count;
+            };
+            for (int chunk = mine > 0 ? kw : chunks; ok && chunk < chunks; chunk += kw_count) {
+                GemvX8<T> xn[HALVES][RT][4];
+#pragma unroll
+                for (int b = 0; b < HALVES; ++b)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            xn[b][r][i].clear();
+                            if (live[r])
+                                xn[b][r][i].load(xr[r], chunk * kChunk + b * 128 + slot_word<GROUP>(t, i) * 8, p.k, x_vec);
+                        }
+#pragma unroll
+                for (int b = 0; b < HALVES; ++b)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) xn[b][r][i].template lay_out<kTerms>(xb[b][r][i]);
+                if (!scales_here) {
+                    ok = __all_sync(~0u, mbar_wait_bounded(&scale_bar, scale_parity, wait_limit_ns, nullptr));
+                    scales_here = true;
                 }
+                int j = 0;
+                for (; ok && j + 2 <= mine; j += 2) {
+                    step_over(std::integral_constant<int, 2>(), j, chunk);
+                    ok = __all_sync(~0u, ok);
+                }
+                if (ok && j < mine) step_over(std::integral_constant<int, 1>(), j, chunk);
+                ok = __all_sync(~0u, ok);
             }
-            __syncthreads();
+            if (!ok && lane == 0) report_status(kStatusTimeoutProducer, nullptr);
+            ok = __syncthreads_and(ok);
+            if (!ok) break;
             const int split = min(kw_count, chunks);
             for (int at = threadIdx.x; at < count * 16 * kCols; at += 32 * kGemvWarps) {
                 const int i = at & 15, rest = at >> 4;  // consecutive threads: consecutive outputs
@@ -515,15 +630,22 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
                 const int out = (m0 + m) * 16 + i;
                 if (c0 + c >= x_count || out >= p.n) continue;
                 const float* v = reinterpret_cast<const float*>(sums + ((m << kw_log) * RT + c / 8) * 32) +
-                                 ((i & 7) * 4 + c % 8 / 2) * 4 + (i >> 3) * 2 + (c & 1);
+                                 (tile_lane<GROUP, HALVES>(i & 7) * 4 + c % 8 / 2) * 4 + (i >> 3) * 2 + (c & 1);
                 float sum = 0.0f;
                 for (int s = 0; s < split; ++s) sum += v[s * RT * 128];
-                y[seg.order[x_first + c0 + c] * ldy + out] = from_f32<T>(sum);
+                y[seg.order[x_first + c0 + c] * ldy + out] = from_f32<T>(sum * (1.0f / Math::kUnit));
             }
             __syncthreads();
         }
+        scale_parity ^= 1;  // one copy of scales per round of tiles
     }
-    if (ids)  // rows of no expert
+    // A wait that gave up leaves copies in flight; they land (or the limit passes) before the block ends.
+    while (!ok && stage != load_stage) {
+        if (!mbar_wait_drain(&bars[warp][stage], parity, wait_limit_ns)) break;
+        if (++stage == kDepth) stage = 0, parity ^= 1;
+    }
+    while (!ok && left > 0 && s_bulk && threadIdx.x == 0 && !mbar_wait_drain(&scale_bar, scale_parity, wait_limit_ns)) break;
+    if (seg.begin[seg.count] < rows)  // rows of no expert
         for (int r = 0; r < rows; ++r) {
             const int e = ids[r];
             if (e >= 0 && e < p.experts) continue;
@@ -532,20 +654,39 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
         }
 }
 
+// Boxes of 16 rows x 64 bytes (or 128) of the codes.
+mfb_status_t encode_codes(CUtensorMap* map, const void* base, long long rows, int row_bytes, int halves) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(MFB_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+    const cuuint32_t box[2] = {64u * halves, 16}, step[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          halves == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(MFB_ECUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string(static_cast<int>(r)) + ")");
+    return MFB_OK;
+}
+
 template <typename T, typename TS, int GROUP>
 mfb_status_t gemv_int4_launch(const Int4Params& p, int device, cudaStream_t stream, int rows, const T* x, long long ldx,
                               const int* ids, T* y, long long ldy) {
     const bool x_vec = (reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * sizeof(T))) % 16 == 0;
-    constexpr int kGroups = 128 / GROUP;
-    const bool s_vec = p.groups % kGroups == 0 && reinterpret_cast<uintptr_t>(p.scales) % (sizeof(TS) * kGroups) == 0 &&
-                       reinterpret_cast<uintptr_t>(p.zeros) % kGroups == 0;
-    const int chunks = (p.k + 127) / 128;
-    int kw_log = 0;
-    while (kw_log < 4 && (1 << kw_log) < chunks) ++kw_log;
+    auto bulk = [&](const void* base, int size) {
+        return aligned16(base) && (p.experts == 1 || static_cast<long long>(p.n) * p.groups * size % 16 == 0);
+    };
+    bool s_bulk = bulk(p.scales, sizeof(TS)) && bulk(p.zeros, 1);
     const long long tiles = static_cast<long long>(ids ? rows : 1) * ((p.n + 15) / 16);
+    if (tiles > 0x7fffffffLL) return fail(MFB_EINVAL, "problem has too many output tiles");
     const unsigned grid = static_cast<unsigned>(std::min<long long>(tiles, sm_count(device)));
-    auto go = [&](auto rt) -> mfb_status_t {
-        const auto kernel = &gemv_int4_kernel<T, TS, GROUP, decltype(rt)::value>;
+    auto go = [&](auto rt, auto halves) -> mfb_status_t {
+        constexpr int RT = decltype(rt)::value, HALVES = decltype(halves)::value;
+        const auto kernel = &gemv_int4_kernel<T, TS, GROUP, RT, HALVES>;
+        const int chunks = (p.k + 128 * HALVES - 1) / (128 * HALVES);
+        CUtensorMap map{};
+        if (p.k > 0) MFB_TRY(encode_codes(&map, p.packed, p.rows, p.row_bytes, HALVES));
         static std::atomic<unsigned long long> raised{0};  // devices whose shared-memory limit is raised
         const unsigned long long bit = 1ull << (device & 63);
         if (!(raised.load(std::memory_order_acquire) & bit)) {
@@ -553,14 +694,36 @@ mfb_status_t gemv_int4_launch(const Int4Params& p, int device, cudaStream_t stre
                          "cudaFuncSetAttribute(gemv_int4)");
             raised.fetch_or(bit, std::memory_order_release);
         }
-        kernel<<<grid, 32 * kGemvWarps, kGemvSmem, stream>>>(p, rows, x, ldx, ids, y, ldy, x_vec, s_vec, kw_log);
+        // Warps along k: the split with the fewest steps per warp; of equal ones the widest whose sums fit at once,
+        // since every further round of tiles starts its loads anew.
+        const long long each = (tiles + grid - 1) / grid;
+        const long long scale_bytes = 16ll * p.groups * (sizeof(TS) + (p.zeros ? 1 : 0));
+        if (scale_bytes > 32768) s_bulk = false;  // rows of millions of columns
+        auto room = [&](int log) {
+            return static_cast<int>((kGemvSmem - kGemvRing) / ((512ll * RT << log) + (s_bulk ? scale_bytes : 0)));
+        };
+        long long best = 0;
+        int kw_log = -1;
+        for (int log = 4; log >= 0; --log) {
+            const long long steps = ((each << log) + kGemvWarps - 1) / kGemvWarps * ((chunks + (1 << log) - 1) >> log);
+            if (kw_log < 0 || steps < best || (steps == best && room(kw_log) < each)) best = steps, kw_log = log;
+        }
+        const int most = room(kw_log);
+        kernel<<<grid, 32 * kGemvWarps, kGemvSmem, stream>>>(map, p, rows, x, ldx, ids, y, ldy, x_vec, s_bulk, kw_log, most,
+                                                             wait_limit_ns());
         MFB_CUDA_TRY(cudaGetLastError(), "gemv_int4 launch");
         return MFB_OK;
     };
-    // Two column tiles of x keep 16 rows in one pass over the codes; FP32 rows have no registers for that.
-    if constexpr (sizeof(T) == 2)
-        if (rows > 8 && !ids) return go(std::integral_constant<int, 2>());
-    return go(std::integral_constant<int, 1>());
+    // Two column tiles of x keep 16 rows in one pass over the codes; FP32 rows have no registers for that, and neither
+    // they nor two tiles for 256 columns of x at a time.
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if constexpr (sizeof(T) == 2) {
+        if (rows > 8 && !ids) return go(Two(), One());
+        return go(One(), Two());
+    } else {
+        return go(One(), One());
+    }
 }
 
 mfb_status_t validate_int4(const mfb_int4_matrix* m, Int4Params* p) {
@@ -581,6 +744,8 @@ mfb_status_t validate_int4(const mfb_int4_matrix* m, Int4Params* p) {
                     static_cast<int>((m->k + static_cast<long long>(m->group) - 1) / m->group),
                     static_cast<int>(row_bytes),
                     m->experts};
+    if (p->rows > INT32_MAX - 65536 || m->k > INT32_MAX - 65536)
+        return fail(MFB_EINVAL, "4-bit matrix dimension exceeds the 32-bit limit");
     if (p->rows == 0 || m->k == 0) return MFB_OK;
     if (!m->packed || !m->scales) return fail(MFB_EINVAL, "null codes or scales of a 4-bit matrix");
     if (!aligned16(m->packed)) return fail(MFB_EINVAL, "packed codes must start on a 16-byte boundary");
