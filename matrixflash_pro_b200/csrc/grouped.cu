@@ -81,11 +81,13 @@ GroupedEntry entry() {
 // Wide tiles on SM pairs, narrow ones on single SMs.
 template <int PLANES, bool RIGHT, bool M_MN, bool TMA>
 GroupedEntry entry_for(bool wide) {
-    if constexpr (PLANES == 1)
-        return wide ? entry<GroupedConfig<256, 2, 1, RIGHT, M_MN, TMA, 6>>() : entry<GroupedConfig<64, 1, 1, RIGHT, M_MN, TMA, 8>>();
+    if constexpr (TMA)
+        return wide ? entry<GroupedConfig<256, 2, 1, RIGHT, M_MN, true, 2, 3>>() : entry<GroupedConfig<64, 1, 1, RIGHT, M_MN, true, 2, 4>>();
+    else if constexpr (PLANES == 1)
+        return wide ? entry<GroupedConfig<256, 2, 1, RIGHT, M_MN, false, 1, 6>>() : entry<GroupedConfig<64, 1, 1, RIGHT, M_MN, false, 1, 8>>();
     else
-        return wide ? entry<GroupedConfig<128, 2, PLANES, RIGHT, M_MN, false, 3>>()
-                    : entry<GroupedConfig<64, 1, PLANES, RIGHT, M_MN, false, 3>>();
+        return wide ? entry<GroupedConfig<128, 2, PLANES, RIGHT, M_MN, false, 1, 3>>()
+                    : entry<GroupedConfig<64, 1, PLANES, RIGHT, M_MN, false, 1, 3>>();
 }
 
 template <int PLANES, bool TMA>

@@ -49,9 +49,11 @@ struct GroupedParams {
     int m_shared;  // all groups share one matrix: the tensor map has one
 };
 
-template <int NT_, int CG_, int PLANES_, bool RIGHT_, bool M_MN_, bool TMA_, int STAGES_>
+// KS = 64-deep slabs per stage. A stage has a fixed cost of a few hundred cycles (barrier wait, commit) beside its
+// MMAs, so four of them (one slab of 16-bit values) are too few.
+template <int NT_, int CG_, int PLANES_, bool RIGHT_, bool M_MN_, bool TMA_, int KS_, int STAGES_>
 struct GroupedConfig {
-    static constexpr int NT = NT_, CG = CG_, PLANES = PLANES_, STAGES = STAGES_;
+    static constexpr int NT = NT_, CG = CG_, PLANES = PLANES_, KS = KS_, STAGES = STAGES_;
     static constexpr bool RIGHT = RIGHT_, TMA = TMA_;
     static constexpr bool M_MN = RIGHT_ || M_MN_;  // M side stored MN-major
     static constexpr bool N_MN = RIGHT_;           // N side stored MN-major
@@ -60,7 +62,8 @@ struct GroupedConfig {
     static constexpr int NTC = NT / CG;  // N-side rows of a CTA
     static constexpr int kMPlane = 128 * 128, kNPlane = NTC * 128;
     static constexpr int kMBytes = PLANES * kMPlane, kNBytes = PLANES * kNPlane;
-    static constexpr int kStage = kMBytes + kNBytes;
+    static constexpr int kSlab = kMBytes + kNBytes;
+    static constexpr int kStage = KS * kSlab;
     static constexpr int kBarriers = STAGES * kStage;
     static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 5) + 16;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
@@ -75,6 +78,7 @@ struct GroupedConfig {
     static constexpr int kFullCount = !TMA ? CG * kLoaders : RIGHT ? CG : 1;
     static_assert(kSmem <= 227 * 1024, "shared memory");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512 && kTmemCols >= 32, "TMEM allocation");
+    static_assert(KS == 1 || (TMA && PLANES == 1), "only TMA stages hold several slabs");
     static_assert(!N_MN || NTC % 64 == 0, "MN-major boxes are 64 columns");
 };
 
@@ -84,7 +88,7 @@ struct GroupedTile {
     int r0, r1;      // output rows [r0, r1)
     int cols;        // N of the MMAs
     int t0, t1;      // gradient: rows contracted over
-    int kb;          // stages
+    int slabs, kb;   // 64-deep slabs of the contraction, and stages
 };
 
 template <class Cfg>
@@ -116,7 +120,8 @@ struct GroupedTiles {
         t.r0 = (Cfg::RIGHT ? 0 : t.t0) + ri;
         t.r1 = t.r0 + left;
         t.cols = (left + Cfg::kGranule - 1) / Cfg::kGranule * Cfg::kGranule;
-        t.kb = ((Cfg::RIGHT ? t.t1 - t.t0 : p.k) + kGroupedDepth - 1) / kGroupedDepth;
+        t.slabs = ((Cfg::RIGHT ? t.t1 - t.t0 : p.k) + kGroupedDepth - 1) / kGroupedDepth;
+        t.kb = (t.slabs + Cfg::KS - 1) / Cfg::KS;
         return true;
     }
 };
@@ -331,13 +336,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         ok = false;
                         break;
                     }
-                    uint8_t* m_tile = smem + s * Cfg::kStage;
-                    uint8_t* n_tile = m_tile + Cfg::kMBytes;
-                    const int d0 = (Cfg::RIGHT ? t.t0 : 0) + kb * kGroupedDepth;
-                    const bool tail = Cfg::RIGHT && d0 + kGroupedDepth > t.t1;
+                    const int slabs = min(Cfg::KS, t.slabs - kb * Cfg::KS);
+                    const bool tail = Cfg::RIGHT && kb == t.kb - 1 && (t.t1 - t.t0) % kGroupedDepth != 0;
                     uint64_t* bar = tail ? &tail_bar[s] : &full_bar[s];
-                    if (tail) mbar_arrive_expect_tx(bar, bytes);
-                    else if (leader) mbar_arrive_expect_tx(bar, CG * bytes);
+                    if (tail) mbar_arrive_expect_tx(bar, slabs * bytes);
+                    else if (leader) mbar_arrive_expect_tx(bar, CG * slabs * bytes);
                     else if (Cfg::kFullCount == CG) arrive_leader(bar);
                     const uint32_t to = map_to_cta(smem_u32(bar), tail ? rank : 0);
                     auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
@@ -345,18 +348,23 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         else tma_load_3d(dst, map, bar, x, y, z);
                     };
                     const int z = Cfg::RIGHT || p.m_shared ? 0 : t.e;
-                    if (Cfg::M_MN) {
-                        load(m_tile, &map_m, f, d0, z);
-                        load(m_tile + 8192, &map_m, f + 64, d0, z);
-                    } else {
-                        load(m_tile, &map_m, d0, f, z);
-                    }
-                    if (Cfg::N_MN) {
-                        for (int b = 0; b < n_rows / 64; ++b) load(n_tile + b * 8192, &map_n, r + 64 * b, d0, 0);
-                    } else if (half == Cfg::NTC) {
-                        load(n_tile, &map_n, d0, r, 0);
-                    } else {
-                        for (int b = 0; b < half / 16; ++b) load(n_tile + b * 2048, &map_n16, d0, r + 16 * b, 0);
+                    for (int j = 0; j < slabs; ++j) {
+                        uint8_t* m_tile = smem + s * Cfg::kStage + j * Cfg::kSlab;
+                        uint8_t* n_tile = m_tile + Cfg::kMBytes;
+                        const int d0 = (Cfg::RIGHT ? t.t0 : 0) + (kb * Cfg::KS + j) * kGroupedDepth;
+                        if (Cfg::M_MN) {
+                            load(m_tile, &map_m, f, d0, z);
+                            load(m_tile + 8192, &map_m, f + 64, d0, z);
+                        } else {
+                            load(m_tile, &map_m, d0, f, z);
+                        }
+                        if (Cfg::N_MN) {
+                            for (int b = 0; b < n_rows / 64; ++b) load(n_tile + b * 8192, &map_n, r + 64 * b, d0, 0);
+                        } else if (half == Cfg::NTC) {
+                            load(n_tile, &map_n, d0, r, 0);
+                        } else {
+                            for (int b = 0; b < half / 16; ++b) load(n_tile + b * 2048, &map_n16, d0, r + 16 * b, 0);
+                        }
                     }
                 }
             }
@@ -472,31 +480,34 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage);
-                    const uint32_t n_addr = m_addr + Cfg::kMBytes;
-                    auto m_desc = [&](int pl, int ks) {
-                        const uint32_t a = m_addr + pl * Cfg::kMPlane;
-                        return Cfg::M_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
-                                         : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
-                    };
-                    auto n_desc = [&](int pl, int ks) {
-                        const uint32_t a = n_addr + pl * Cfg::kNPlane;
-                        return Cfg::N_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
-                                         : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
-                    };
-                    auto mma = [&](int mp, int np, int ks) {
-                        if (CG == 2) umma_f16_pair(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
-                        else umma_f16(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
-                        acc = 1;
-                    };
-                    // The small products of all steps first: every addition truncates relative to what the
-                    // accumulator holds, so only the last four cut at the sum's own size.
-                    constexpr int kTerms = PLANES == 3 ? 6 : PLANES == 2 ? 3 : 1;
-                    constexpr int kMTerm[6] = {2, 0, 1, 1, 0, 0}, kNTerm[6] = {0, 2, 1, 0, 1, 0};
+                    const int slabs = Cfg::KS == 1 ? 1 : min(Cfg::KS, t.slabs - kb * Cfg::KS);
+                    for (int j = 0; j < slabs; ++j) {
+                        const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage + j * Cfg::kSlab);
+                        const uint32_t n_addr = m_addr + Cfg::kMBytes;
+                        auto m_desc = [&](int pl, int ks) {
+                            const uint32_t a = m_addr + pl * Cfg::kMPlane;
+                            return Cfg::M_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
+                                             : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
+                        };
+                        auto n_desc = [&](int pl, int ks) {
+                            const uint32_t a = n_addr + pl * Cfg::kNPlane;
+                            return Cfg::N_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
+                                             : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
+                        };
+                        auto mma = [&](int mp, int np, int ks) {
+                            if (CG == 2) umma_f16_pair(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
+                            else umma_f16(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
+                            acc = 1;
+                        };
+                        // The small products of all steps first: every addition truncates relative to what the
+                        // accumulator holds, so only the last four cut at the sum's own size.
+                        constexpr int kTerms = PLANES == 3 ? 6 : PLANES == 2 ? 3 : 1;
+                        constexpr int kMTerm[6] = {2, 0, 1, 1, 0, 0}, kNTerm[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-                    for (int i = 6 - kTerms; i < 6; ++i)
+                        for (int i = 6 - kTerms; i < 6; ++i)
 #pragma unroll
-                        for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                            for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                    }
                     if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
                     else umma_commit(&empty_bar[s]);
                     if (PLANES == 3 || kb == t.kb - 1) {
@@ -529,7 +540,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 break;
             }
             phases ^= 1u << s;
-            const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
+            const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage + (t.slabs - 1) % Cfg::KS * Cfg::kSlab);
             const int boxes = (t.cols / CG + 63) / 64;
             for (int b = 0; b < 2 + boxes; ++b) {
                 const uint32_t box = m_tile + (b < 2 ? b * 8192 : Cfg::kMBytes + (b - 2) * 8192);
