@@ -193,18 +193,18 @@ mfb_status_t launch_grouped(int device, const mfb_grouped_desc& d, cudaStream_t 
                                       : (d.rows + e.nt - 1) / e.nt + std::min(d.groups, d.rows);
     if (row_tiles * p.m_tiles > 0x7fffffffLL) return fail(MFB_EINVAL, "problem has too many output tiles");
 
-    CUtensorMap maps[3] = {};
+    CUtensorMap maps[4] = {};
     if (tma) {
         if (right) {
             MFB_TRY(encode_16bit(&maps[0], b, d.rows, d.n, d.ldb, 1, 0, 64));
             MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, 64));
-            maps[2] = maps[1];
         } else {
             const long long b_rows = d.trans_b ? d.n : d.k;
             const int b_cols = d.trans_b ? d.k : d.n;
             MFB_TRY(encode_16bit(&maps[0], b, b_rows, b_cols, d.ldb, shared ? 1 : d.groups, d.stride, m_mn ? 64 : 128));
             MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, e.nt / e.cg));
-            MFB_TRY(encode_16bit(&maps[2], a, d.rows, d.k, d.lda, 1, 0, 16));
+            MFB_TRY(encode_16bit(&maps[2], a, d.rows, d.k, d.lda, 1, 0, 32));
+            MFB_TRY(encode_16bit(&maps[3], a, d.rows, d.k, d.lda, 1, 0, 16));
         }
     }
     int workers = 0;
@@ -212,7 +212,7 @@ mfb_status_t launch_grouped(int device, const mfb_grouped_desc& d, cudaStream_t 
     // Without tiles the launch still clears the rows of no group.
     const long long useful = std::max(row_tiles * p.m_tiles, d.zero_rest ? (d.rows + 7ll) / 8 : 1ll);
     workers = static_cast<int>(std::min<long long>(workers, useful));
-    void* args[] = {&maps[0], &maps[1], &maps[2], &p};
+    void* args[] = {&maps[0], &maps[1], &maps[2], &maps[3], &p};
     cudaLaunchConfig_t lc{};
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;

@@ -11,7 +11,7 @@
 // group), and its roles walk the same tile sequence, dealt out round-robin to the persistent workers.
 //
 // 16-bit operands whose rows TMA can address come by TMA, 64 of the contraction deep, 128-byte swizzle
-// (K-major tiles one box or boxes of 16 rows; MN-major tiles boxes of 64 columns). All others (FP32, odd
+// (K-major tiles one box, or boxes of 32 and 16 rows; MN-major tiles boxes of 64 columns). All others (FP32, odd
 // strides) come by eight loader warps that read global memory into registers and write the same layout:
 // 16-bit values as they are, FP32 as PLANES BF16 terms x = h + m + l (h cut, m and l rounded; exact with
 // three). Products hh, hm, mh, mm, hl, lh are kept (six MMAs per step, 1/6 of the BF16 rate); what is left
@@ -217,7 +217,8 @@ struct GroupedChunk {
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n,
-                      const __grid_constant__ CUtensorMap map_n16, const GroupedParams p) {
+                      const __grid_constant__ CUtensorMap map_n32, const __grid_constant__ CUtensorMap map_n16,
+                      const GroupedParams p) {
     constexpr int NT = Cfg::NT, CG = Cfg::CG, PLANES = Cfg::PLANES, STAGES = Cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -363,7 +364,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         } else if (half == Cfg::NTC) {
                             load(n_tile, &map_n, d0, r, 0);
                         } else {
-                            for (int b = 0; b < half / 16; ++b) load(n_tile + b * 2048, &map_n16, d0, r + 16 * b, 0);
+                            int row = 0;
+                            for (; row + 32 <= half; row += 32) load(n_tile + row * 128, &map_n32, d0, r + row, 0);
+                            if (row < half) load(n_tile + row * 128, &map_n16, d0, r + row, 0);
                         }
                     }
                 }
