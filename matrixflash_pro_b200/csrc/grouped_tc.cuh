@@ -67,7 +67,7 @@ struct GroupedConfig {
     static constexpr int kBarriers = STAGES * kStage;
     static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 5) + 16;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
-    static constexpr int kLoaders = TMA ? 1 : 8;  // warps
+    static constexpr int kLoaders = TMA ? 2 : 8;  // warps; TMA: one per operand
     static constexpr int kMmaWarp = kLoaders, kFixWarp = kLoaders + 1;
     static constexpr int kEpiWarp0 = TMA && RIGHT ? kLoaders + 2 : kLoaders + 1;
     static constexpr int kEpiWarps = 8;
@@ -126,10 +126,39 @@ struct GroupedTiles {
     }
 };
 
+template <typename T>
+__device__ __forceinline__ T grouped_round(float v);
+template <>
+__device__ __forceinline__ float grouped_round<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ __half grouped_round<__half>(float v) {
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 grouped_round<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
 __device__ __forceinline__ void grouped_store(const GroupedParams& p, long long at, float v) {
     if (p.out_f32) static_cast<float*>(p.c)[at] = v;
     else if (p.bf16) static_cast<__nv_bfloat16*>(p.c)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(p.c)[at] = __float2half_rn(v);
+}
+
+// Rows [first, first + 16) of a column, as far as there are `rows`; `at` is row 0's place.
+template <typename T>
+__device__ __forceinline__ void grouped_store16(const GroupedParams& p, long long at, int first, int rows, const float (&v)[16]) {
+    T* to = static_cast<T*>(p.c) + at + first * p.ldc;
+    if (first + 16 <= rows) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, to += p.ldc) *to = grouped_round<T>(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, to += p.ldc)
+            if (first + j < rows) *to = grouped_round<T>(v[j]);
+    }
 }
 
 // Eight consecutive elements of a row in global memory; zeros outside [.., rows) x [.., cols).
@@ -320,8 +349,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         else mbar_arrive(bar);
     };
 
-    if (Cfg::TMA && warp == 0) {
-        // ------------------------------------------------------------ TMA producer
+    if (Cfg::TMA && warp < 2) {
+        // ------------------------------------------------------------ TMA producers: M side, N side
+        // Issuing copies is what a producer spends its time on, so each operand has its own; the M side's posts the
+        // bytes of both.
         if (lane == 0) {
             int it = 0;
             bool ok = true;
@@ -340,9 +371,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     const int slabs = min(Cfg::KS, t.slabs - kb * Cfg::KS);
                     const bool tail = Cfg::RIGHT && kb == t.kb - 1 && (t.t1 - t.t0) % kGroupedDepth != 0;
                     uint64_t* bar = tail ? &tail_bar[s] : &full_bar[s];
-                    if (tail) mbar_arrive_expect_tx(bar, slabs * bytes);
-                    else if (leader) mbar_arrive_expect_tx(bar, CG * slabs * bytes);
-                    else if (Cfg::kFullCount == CG) arrive_leader(bar);
+                    if (warp == 0) {
+                        if (tail) mbar_arrive_expect_tx(bar, slabs * bytes);
+                        else if (leader) mbar_arrive_expect_tx(bar, CG * slabs * bytes);
+                        else if (Cfg::kFullCount == CG) arrive_leader(bar);
+                    }
                     const uint32_t to = map_to_cta(smem_u32(bar), tail ? rank : 0);
                     auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
                         if (CG == 2) tma_load_3d_pair(dst, map, to, x, y, z);
@@ -353,13 +386,14 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         uint8_t* m_tile = smem + s * Cfg::kStage + j * Cfg::kSlab;
                         uint8_t* n_tile = m_tile + Cfg::kMBytes;
                         const int d0 = (Cfg::RIGHT ? t.t0 : 0) + (kb * Cfg::KS + j) * kGroupedDepth;
-                        if (Cfg::M_MN) {
-                            load(m_tile, &map_m, f, d0, z);
-                            load(m_tile + 8192, &map_m, f + 64, d0, z);
-                        } else {
-                            load(m_tile, &map_m, d0, f, z);
-                        }
-                        if (Cfg::N_MN) {
+                        if (warp == 0) {
+                            if (Cfg::M_MN) {
+                                load(m_tile, &map_m, f, d0, z);
+                                load(m_tile + 8192, &map_m, f + 64, d0, z);
+                            } else {
+                                load(m_tile, &map_m, d0, f, z);
+                            }
+                        } else if (Cfg::N_MN) {
                             for (int b = 0; b < n_rows / 64; ++b) load(n_tile + b * 8192, &map_n, r + 64 * b, d0, 0);
                         } else if (half == Cfg::NTC) {
                             load(n_tile, &map_n, d0, r, 0);
@@ -565,9 +599,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             const long long at = (Cfg::RIGHT ? t.e * p.stride_c : 0) + t.r0 * p.ldc + f;
             const int rows = f < p.n ? t.r1 - t.r0 : 0;  // this lane's column of each row
             auto store = [&](int q, const float (&v)[16]) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (q * 16 + j < rows) grouped_store(p, at + (q * 16 + j) * p.ldc, v[j]);
+                if (p.out_f32) grouped_store16<float>(p, at, q * 16, rows, v);
+                else if (p.bf16) grouped_store16<__nv_bfloat16>(p, at, q * 16, rows, v);
+                else grouped_store16<__half>(p, at, q * 16, rows, v);
             };
             if (t.kb == 0) {
                 const float zero[16] = {};
