@@ -65,7 +65,7 @@ struct GroupedConfig {
     static constexpr int kSlab = kMBytes + kNBytes;
     static constexpr int kStage = KS * kSlab;
     static constexpr int kBarriers = STAGES * kStage;
-    static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 5) + 16;
+    static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 6) + 8;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
     static constexpr int kLoaders = TMA ? 2 : 8;  // warps; TMA: one per operand
     static constexpr int kMmaWarp = kLoaders, kFixWarp = kLoaders + 1;
@@ -75,7 +75,7 @@ struct GroupedConfig {
     static constexpr int kTmemCols = 2 * NT;
     static constexpr int kGranule = 16 * CG;  // N of an MMA is a multiple of this
     // Arrivals that complete a filled stage, besides the bytes of TMA copies.
-    static constexpr int kFullCount = !TMA ? CG * kLoaders : RIGHT ? CG : 1;
+    static constexpr int kFullCount = !TMA ? CG * kLoaders : 1;
     static_assert(kSmem <= 227 * 1024, "shared memory");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512 && kTmemCols >= 32, "TMEM allocation");
     static_assert(KS == 1 || (TMA && PLANES == 1), "only TMA stages hold several slabs");
@@ -88,7 +88,7 @@ struct GroupedTile {
     int r0, r1;      // output rows [r0, r1)
     int cols;        // N of the MMAs
     int t0, t1;      // gradient: rows contracted over
-    int slabs, kb;   // 64-deep slabs of the contraction, and stages
+    int steps, slabs, kb;  // 16-deep MMA steps and 64-deep slabs of the contraction, and stages
 };
 
 template <class Cfg>
@@ -120,7 +120,8 @@ struct GroupedTiles {
         t.r0 = (Cfg::RIGHT ? 0 : t.t0) + ri;
         t.r1 = t.r0 + left;
         t.cols = (left + Cfg::kGranule - 1) / Cfg::kGranule * Cfg::kGranule;
-        t.slabs = ((Cfg::RIGHT ? t.t1 - t.t0 : p.k) + kGroupedDepth - 1) / kGroupedDepth;
+        t.steps = ((Cfg::RIGHT ? t.t1 - t.t0 : p.k) + 15) / 16;
+        t.slabs = (t.steps + kGroupedDepth / 16 - 1) / (kGroupedDepth / 16);
         t.kb = (t.slabs + Cfg::KS - 1) / Cfg::KS;
         return true;
     }
@@ -257,7 +258,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     uint64_t* acc_full_bar = tail_bar + STAGES;
     uint64_t* acc_empty_bar = acc_full_bar + 2;  // used in the leader
     uint64_t* drain_bar = acc_empty_bar + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+    uint64_t* peer_tail_bar = drain_bar + 1;  // in the leader: the peer's tail is cleared
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(peer_tail_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* offset = reinterpret_cast<int*>(smem + Cfg::kTables);
     int* first_tile = offset + kGroupedMaxGroups + 1;
@@ -279,6 +281,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             mbar_init(&acc_empty_bar[b], CG * Cfg::kEpiWarps);
         }
         mbar_init(drain_bar, 1);
+        mbar_init(peer_tail_bar, 1);
         *abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async_smem();
@@ -369,12 +372,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         break;
                     }
                     const int slabs = min(Cfg::KS, t.slabs - kb * Cfg::KS);
-                    const bool tail = Cfg::RIGHT && kb == t.kb - 1 && (t.t1 - t.t0) % kGroupedDepth != 0;
+                    const bool tail = Cfg::RIGHT && kb == t.kb - 1 && (t.t1 - t.t0) % 16 != 0;
                     uint64_t* bar = tail ? &tail_bar[s] : &full_bar[s];
                     if (warp == 0) {
                         if (tail) mbar_arrive_expect_tx(bar, slabs * bytes);
                         else if (leader) mbar_arrive_expect_tx(bar, CG * slabs * bytes);
-                        else if (Cfg::kFullCount == CG) arrive_leader(bar);
                     }
                     const uint32_t to = map_to_cta(smem_u32(bar), tail ? rank : 0);
                     auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
@@ -519,6 +521,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     tc_fence_after();
                     const int slabs = Cfg::KS == 1 ? 1 : min(Cfg::KS, t.slabs - kb * Cfg::KS);
                     for (int j = 0; j < slabs; ++j) {
+                        // 16-deep steps of this slab that the contraction still has
+                        const int steps = min(kGroupedDepth / 16, t.steps - (kb * Cfg::KS + j) * (kGroupedDepth / 16));
                         const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage + j * Cfg::kSlab);
                         const uint32_t n_addr = m_addr + Cfg::kMBytes;
                         auto m_desc = [&](int pl, int ks) {
@@ -543,7 +547,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 #pragma unroll
                         for (int i = 6 - kTerms; i < 6; ++i)
 #pragma unroll
-                            for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                            for (int ks = 0; ks < kGroupedDepth / 16; ++ks)
+                                if (ks < steps) mma(kMTerm[i], kNTerm[i], ks);
                     }
                     if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
                     else umma_commit(&empty_bar[s]);
@@ -560,15 +565,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (Cfg::TMA && Cfg::RIGHT && warp == Cfg::kFixWarp) {
         // ------------------------------------------------------------ clears the rows behind a group
-        // The last stage of a contraction over a group's rows holds rows of the next group (or NaN of a
-        // buffer's spare rows): both operands' tails become 0 before the MMA may read them.
+        // The last MMA step of a contraction over a group's rows may hold rows of the next group (or NaN of a
+        // buffer's spare rows): both operands' become 0 before the MMA may read them.
         int it = 0;
-        uint32_t phases = 0;  // parity of each stage's tail barrier
+        uint32_t phases = 0, peer_phase = 0;  // parities of each stage's tail barrier, of the peer's
         bool ok = true;
         while (ok && work.next(t)) {
-            const int valid = (t.t1 - t.t0) % kGroupedDepth;
+            const int rows = t.t1 - t.t0, valid = rows % kGroupedDepth, end = (valid + 15) / 16 * 16;
             it += t.kb;
-            if (valid == 0) continue;
+            if (rows % 16 == 0) continue;
             const int s = (it - 1) % STAGES;
             ok = mbar_wait_bounded(&tail_bar[s], (phases >> s) & 1, limit, abort_flag);
             ok = __all_sync(~0u, ok);
@@ -581,11 +586,24 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             const int boxes = (t.cols / CG + 63) / 64;
             for (int b = 0; b < 2 + boxes; ++b) {
                 const uint32_t box = m_tile + (b < 2 ? b * 8192 : Cfg::kMBytes + (b - 2) * 8192);
-                for (int at = valid * 128 + lane * 16; at < 8192; at += 512) GroupedChunk<2>::st(box + at, 0, 0, 0, 0);
+                for (int at = valid * 128 + lane * 16; at < end * 128; at += 512) GroupedChunk<2>::st(box + at, 0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) arrive_leader(&full_bar[s]);
+            // One arrival completes the stage: the leader's, after the peer's tail is cleared too.
+            if (CG == 2 && !leader) {
+                if (lane == 0) mbar_arrive_cluster(leader_bar(peer_tail_bar));
+                continue;
+            }
+            if (CG == 2) {
+                ok = __all_sync(~0u, mbar_wait_bounded(peer_tail_bar, peer_phase, limit, abort_flag));
+                peer_phase ^= 1;
+                if (!ok) {
+                    if (lane == 0) give_up(kStatusTimeoutProducer);
+                    break;
+                }
+            }
+            if (lane == 0) mbar_arrive(&full_bar[s]);
         }
     } else if (warp >= Cfg::kEpiWarp0) {
         // ------------------------------------------------------------ epilogue
