@@ -74,8 +74,9 @@ struct GroupedConfig {
     static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
     static constexpr int kTmemCols = 2 * NT;
     static constexpr int kGranule = 16 * CG;  // N of an MMA is a multiple of this
-    // Arrivals that complete a filled stage, besides the bytes of TMA copies.
-    static constexpr int kFullCount = !TMA ? CG * kLoaders : 1;
+    // Arrivals that complete a filled stage, besides the bytes of TMA copies: the loader warps', and in the leader of
+    // a pair one from the peer. (An arrival across the pair is slow, so the peer's idle MMA warp makes it.)
+    __device__ static int full_count(bool leader) { return TMA ? 1 : kLoaders + (CG == 2 && leader ? 1 : 0); }
     static_assert(kSmem <= 227 * 1024, "shared memory");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512 && kTmemCols >= 32, "TMEM allocation");
     static_assert(KS == 1 || (TMA && PLANES == 1), "only TMA stages hold several slabs");
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     constexpr int NT = Cfg::NT, CG = Cfg::CG, PLANES = Cfg::PLANES, STAGES = Cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kBarriers);  // used in the leader
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kBarriers);  // of the leader: both CTAs' stage is filled
     uint64_t* empty_bar = full_bar + STAGES;
     uint64_t* tail_bar = empty_bar + STAGES;  // a stage whose last rows are still to be cleared
     uint64_t* acc_full_bar = tail_bar + STAGES;
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full_bar[s], Cfg::kFullCount);
+            mbar_init(&full_bar[s], Cfg::full_count(leader));
             mbar_init(&empty_bar[s], 1);
             mbar_init(&tail_bar[s], 1);
         }
@@ -488,7 +489,24 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 if (kb + 1 < t.kb) load_n(kb + 1);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive_leader(&full_bar[s]);
+                if (lane == 0) mbar_arrive(&full_bar[s]);
+            }
+        }
+    } else if (!Cfg::TMA && CG == 2 && warp == Cfg::kMmaWarp && !leader) {
+        // ------------------------------------------------------------ tells the leader of the peer's filled stages
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            while (ok && work.next(t)) {
+                for (int kb = 0; kb < t.kb; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait_bounded(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
+                        give_up(kStatusTimeoutProducer);
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_cluster(leader_bar(&full_bar[s]));
+                }
             }
         }
     } else if (warp == Cfg::kMmaWarp) {
