@@ -163,52 +163,61 @@ __device__ __forceinline__ void grouped_store16(const GroupedParams& p, long lon
     }
 }
 
-// Eight consecutive elements of a row in global memory; zeros outside [.., rows) x [.., cols).
+// Eight consecutive elements of a row in global memory.
 template <int ES>
 struct GroupedChunk {
     uint32_t w[2 * ES];  // ES 2: four words of two values; ES 4: eight FP32 values
 
-    __device__ __forceinline__ void load(const char* base, long long ld, int align, int row, int rows, int col,
-                                         int cols) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < 2 * ES; ++i) w[i] = 0;
+    }
+
+    // All eight are there; `align`: bytes that the address is a multiple of.
+    __device__ __forceinline__ void load(const char* src, int align) {
+        if (align >= 16) {
+            if (ES == 4 && align >= 32) {
+                asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4 % (2 * ES)]), "=r"(w[5 % (2 * ES)]),
+                               "=r"(w[6 % (2 * ES)]), "=r"(w[7 % (2 * ES)])
+                             : "l"(src));
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < ES / 2; ++i) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+        } else if (ES == 4 || align >= 4) {
+#pragma unroll
+            for (int i = 0; i < 2 * ES; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+        } else {
+            // Rows start at any even address: the aligned words between the first and the last value.
+            const bool odd = reinterpret_cast<uintptr_t>(src) & 2;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(src + (odd ? 2 : 0));
+            const uint32_t edge = __ldg(reinterpret_cast<const uint16_t*>(src) + (odd ? 0 : 6));
+            const uint32_t last = __ldg(reinterpret_cast<const uint16_t*>(src) + 7);
+            const uint32_t v0 = __ldg(words), v1 = __ldg(words + 1), v2 = __ldg(words + 2);
+            w[0] = odd ? edge | v0 << 16 : v0;
+            w[1] = odd ? __funnelshift_r(v0, v1, 16) : v1;
+            w[2] = odd ? __funnelshift_r(v1, v2, 16) : v2;
+            w[3] = odd ? v2 >> 16 | last << 16 : edge | last << 16;
+        }
+    }
+
+    // Those in [.., rows) x [.., cols), zeros for the others.
+    __device__ __forceinline__ void load_some(const char* base, long long ld, int align, int row, int rows, int col,
+                                              int cols) {
+        clear();
         if (row >= rows || col >= cols) return;
         const char* src = base + row * ld + static_cast<long long>(col) * ES;
         if (col + 8 <= cols) {
-            if (align >= 16) {
-#pragma unroll
-                for (int i = 0; i < ES / 2; ++i) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-                    w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-                }
-                return;
-            }
-            if (align >= 4) {
-#pragma unroll
-                for (int i = 0; i < 2 * ES; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
-                return;
-            }
-            if (ES == 2) {  // rows start at any even address
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-                if (reinterpret_cast<uintptr_t>(src) & 2) {
-                    const uint32_t first = __ldg(h), last = __ldg(h + 7);
-                    uint32_t v[3];
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) v[i] = __ldg(reinterpret_cast<const uint32_t*>(h + 1) + i);
-                    w[0] = first | v[0] << 16;
-                    w[1] = v[0] >> 16 | v[1] << 16;
-                    w[2] = v[1] >> 16 | v[2] << 16;
-                    w[3] = v[2] >> 16 | last << 16;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
-                }
-                return;
-            }
+            load(src, align);
+            return;
         }
-        const int count = min(8, cols - col);
+        const int count = cols - col;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 7; ++i) {
             if (i >= count) continue;
             if (ES == 2)
                 w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + i)) << (16 * (i % 2));
@@ -227,7 +236,7 @@ struct GroupedChunk {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float lo = __uint_as_float(w[2 * i]), hi = __uint_as_float(w[2 * i + 1]);
-                asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(t[0][i]) : "f"(hi), "f"(lo));
+                t[0][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);  // cut to the upper halves
 #pragma unroll
                 for (int pl = 1; pl < PLANES; ++pl) {
                     lo -= __uint_as_float(t[pl - 1][i] << 16);
@@ -242,6 +251,76 @@ struct GroupedChunk {
 
     __device__ __forceinline__ static void st(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    }
+};
+
+// One operand's 64-deep slabs on the way from global memory through registers into shared memory: WIDTH rows of the
+// tile (columns, where the operand is MN-major). A thread's chunks are 32 rows apart (K-major: 8 chunks a row) or
+// 256 / (WIDTH / 8) rows of the contraction (MN-major).
+template <class Cfg, int WIDTH, bool MN>
+struct GroupedSide {
+    static constexpr int ES = Cfg::ES, kThreads = 32 * Cfg::kLoaders;
+    static constexpr int kPerRow = MN ? WIDTH / 8 : 8;
+    static constexpr int kChunks = (WIDTH * 8 + kThreads - 1) / kThreads;
+    static constexpr int kApart = kThreads / kPerRow;  // rows between a thread's chunks
+    static constexpr int kPlane = WIDTH * 128;
+    GroupedChunk<ES> c[kChunks];
+    const char* base;
+    const char* at[MN ? 1 : kChunks];  // this thread's chunks of the next slab
+    long long ld;
+    int align, first, width, last, d0, d1;
+    bool inside;
+
+    // Rows (columns) [first_, first_ + width_) of the operand, which ends at last_; contraction [d0_, d1_).
+    __device__ __forceinline__ void start(const char* base_, long long ld_, int align_, int first_, int width_, int last_,
+                                          int d0_, int d1_, int id) {
+        base = base_, ld = ld_, align = align_, first = first_, width = width_, last = last_, d0 = d0_, d1 = d1_;
+        inside = MN ? first + WIDTH <= last : first < last;
+        if (MN) {
+            at[0] = base + (d0 + id / kPerRow) * ld + static_cast<long long>(first + id % kPerRow * 8) * ES;
+        } else {
+#pragma unroll
+            for (int i = 0; i < (MN ? 1 : kChunks); ++i)  // rows past the end repeat the last: their results go nowhere
+                at[i] = base + min(first + i * kApart + id / 8, last - 1) * ld + static_cast<long long>(d0 + id % 8 * 8) * ES;
+        }
+    }
+
+    __device__ __forceinline__ bool has(int i, int id) const {  // whether chunk i is one of the tile's
+        return (WIDTH * 8) % kThreads == 0 || i * kThreads + id < WIDTH * 8;
+    }
+
+    __device__ __forceinline__ void load(int id) {
+        if (inside && d0 + kGroupedDepth <= d1) {
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                if (!has(i, id)) continue;
+                if (MN) {
+                    c[i].load(at[0] + i * kApart * ld, align);
+                } else if (i * kApart < width) {
+                    c[i].load(at[i], align);
+                    at[i] += kGroupedDepth * ES;
+                }
+            }
+            if (MN) at[0] += kGroupedDepth * ld;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                if (!has(i, id)) continue;
+                const int row = i * kApart + id / kPerRow, col = id % kPerRow * 8;
+                if (MN) c[i].load_some(base, ld, align, d0 + row, d1, first + col, last);
+                else c[i].load_some(base, ld, align, first + row, last, d0 + col, d1);
+            }
+        }
+        d0 += kGroupedDepth;
+    }
+
+    __device__ __forceinline__ void store(uint32_t tile, int id) const {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (!has(i, id) || (!MN && i * kApart >= width)) continue;
+            const int row = i * kApart + id / kPerRow, col = id % kPerRow, box = MN ? col / 8 : 0;
+            c[i].template store<Cfg::PLANES>(tile + box * 8192 + row * 128 + (((col % 8) ^ (row & 7)) << 4), kPlane);
+        }
     }
 };
 
@@ -418,47 +497,24 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (!Cfg::TMA && warp < Cfg::kLoaders) {
         // ------------------------------------------------------------ loader warps
-        constexpr int ES = Cfg::ES;
-        constexpr int kThreads = 32 * Cfg::kLoaders;
-        constexpr int kM = 1024 / kThreads, kN = (Cfg::NTC * 8 + kThreads - 1) / kThreads;  // chunks per thread
-        GroupedChunk<ES> cm[kM], cn[kN];
+        // A slab's chunks of eight elements are dealt out to the threads; each keeps the next slab's in registers while
+        // it writes this one's. Where a slab lies inside the operand (all but edges) a chunk costs a pointer step and
+        // its loads.
+        using M = GroupedSide<Cfg, 128, Cfg::M_MN>;
+        using N = GroupedSide<Cfg, Cfg::NTC, Cfg::N_MN>;
+        M m;
+        N n;
         const int id = threadIdx.x;
         int it = 0;
         bool ok = true;
         while (ok && work.next(t)) {
             const int half = t.cols / CG;
-            const int f = t.f0 + 128 * rank, r = t.r0 + half * rank;
-            const char* mb = p.m_base + (Cfg::RIGHT ? 0 : t.e * p.m_stride);
-            const int depth_end = Cfg::RIGHT ? t.t1 : p.k;
-            const int r_end = Cfg::RIGHT ? p.k : t.t1;
-            auto load_m = [&](int kb) {
-                const int d0 = (Cfg::RIGHT ? t.t0 : 0) + kb * kGroupedDepth;
-#pragma unroll
-                for (int i = 0; i < kM; ++i) {
-                    const int q = i * kThreads + id;
-                    if (Cfg::M_MN)
-                        cm[i].load(mb, p.m_ld, p.m_align, d0 + q / 16, depth_end, f + q % 16 * 8, p.n);
-                    else
-                        cm[i].load(mb, p.m_ld, p.m_align, f + q / 8, p.n, d0 + q % 8 * 8, depth_end);
-                }
-            };
-            auto load_n = [&](int kb) {
-                const int d0 = (Cfg::RIGHT ? t.t0 : 0) + kb * kGroupedDepth;
-#pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    const int q = i * kThreads + id;
-                    constexpr int kRow = Cfg::NTC / 8;  // chunks of an MN-major row
-                    if (Cfg::N_MN)
-                        cn[i].load(p.n_base, p.n_ld, p.n_align, d0 + q / kRow, depth_end, r + q % kRow * 8,
-                                   q % kRow * 8 < half ? r_end : 0);
-                    else
-                        cn[i].load(p.n_base, p.n_ld, p.n_align, r + q / 8, q / 8 < half ? r_end : 0, d0 + q % 8 * 8,
-                                   depth_end);
-                }
-            };
+            const int d0 = Cfg::RIGHT ? t.t0 : 0, d1 = Cfg::RIGHT ? t.t1 : p.k;
+            m.start(p.m_base + (Cfg::RIGHT ? 0 : t.e * p.m_stride), p.m_ld, p.m_align, t.f0 + 128 * rank, 128, p.n, d0, d1, id);
+            n.start(p.n_base, p.n_ld, p.n_align, t.r0 + half * rank, half, Cfg::RIGHT ? p.k : t.t1, d0, d1, id);
             if (t.kb > 0) {
-                load_m(0);
-                load_n(0);
+                m.load(id);
+                n.load(id);
             }
             for (int kb = 0; kb < t.kb; ++kb, ++it) {
                 const int s = it % STAGES;
@@ -469,24 +525,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     break;
                 }
                 const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
-                const uint32_t n_tile = m_tile + Cfg::kMBytes;
-#pragma unroll
-                for (int i = 0; i < kM; ++i) {
-                    const int q = i * kThreads + id;
-                    const int row = Cfg::M_MN ? q / 16 : q / 8, c = q % 8, box = Cfg::M_MN ? q % 16 / 8 : 0;
-                    cm[i].template store<PLANES>(m_tile + box * 8192 + row * 128 + ((c ^ (row & 7)) << 4), Cfg::kMPlane);
-                }
-                if (kb + 1 < t.kb) load_m(kb + 1);
-#pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    const int q = i * kThreads + id;
-                    constexpr int kRow = Cfg::NTC / 8;
-                    const int row = Cfg::N_MN ? q / kRow : q / 8, c = q % 8, box = Cfg::N_MN ? q % kRow / 8 : 0;
-                    if ((Cfg::NTC * 8) % kThreads == 0 || q < Cfg::NTC * 8)
-                        cn[i].template store<PLANES>(n_tile + box * 8192 + row * 128 + ((c ^ (row & 7)) << 4),
-                                                     Cfg::kNPlane);
-                }
-                if (kb + 1 < t.kb) load_n(kb + 1);
+                m.store(m_tile, id);
+                if (kb + 1 < t.kb) m.load(id);
+                n.store(m_tile + Cfg::kMBytes, id);
+                if (kb + 1 < t.kb) n.load(id);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full_bar[s]);
