@@ -128,22 +128,26 @@ mfb_status_t grouped_workers(const GroupedEntry& e, int device, int* out) {
     return MFB_OK;
 }
 
-// Tensor map over `count` matrices of 16-bit elements, boxes of 64 columns.
+// Tensor map over `count` matrices of 16-bit elements: boxes of 64 columns x box_rows, or with `wide` boxes > 0 (cols
+// a multiple of 64) `wide` such boxes side by side, the columns as an axis of 64 and one of boxes.
 mfb_status_t encode_16bit(CUtensorMap* map, const void* base, long long rows, int cols, long long ld, long long count,
-                          long long stride, int box_rows) {
+                          long long stride, int box_rows, int wide = 0) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail(MFB_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
-                                static_cast<cuuint64_t>(count)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(count > 1 ? stride : ld) * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
-    const cuuint32_t step[3] = {1, 1, 1};
+    const cuuint64_t row_bytes = static_cast<cuuint64_t>(ld) * 2;
+    const cuuint64_t matrix_bytes = static_cast<cuuint64_t>(count > 1 ? stride : ld) * 2;
+    const cuuint64_t r = static_cast<cuuint64_t>(rows), n = static_cast<cuuint64_t>(count);
+    const cuuint32_t br = static_cast<cuuint32_t>(box_rows), step[4] = {1, 1, 1, 1};
+    const cuuint64_t dims3[3] = {static_cast<cuuint64_t>(cols), r, n}, strides3[2] = {row_bytes, matrix_bytes};
+    const cuuint64_t dims4[4] = {64, r, static_cast<cuuint64_t>(cols / 64), n}, strides4[3] = {row_bytes, 128, matrix_bytes};
+    const cuuint32_t box3[3] = {64, br, 1}, box4[4] = {64, br, static_cast<cuuint32_t>(wide), 1};
     // The bits are copied as they are, FP16 or BF16.
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return fail(MFB_ECUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string(static_cast<int>(r)) + ")");
+    const CUresult result =
+        fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, wide ? 4 : 3, const_cast<void*>(base), wide ? dims4 : dims3,
+           wide ? strides4 : strides3, wide ? box4 : box3, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (result != CUDA_SUCCESS)
+        return fail(MFB_ECUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string(static_cast<int>(result)) + ")");
     return MFB_OK;
 }
 
@@ -195,14 +199,17 @@ mfb_status_t launch_grouped(int device, const mfb_grouped_desc& d, cudaStream_t 
 
     CUtensorMap maps[4] = {};
     if (tma) {
+        p.m_wide = m_mn && d.n % 64 == 0;
+        p.n_wide = right && d.k % 64 == 0;
+        const int m_wide = p.m_wide ? 2 : 0, n_box = e.nt / e.cg;
         if (right) {
-            MFB_TRY(encode_16bit(&maps[0], b, d.rows, d.n, d.ldb, 1, 0, 64));
-            MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, 64));
+            MFB_TRY(encode_16bit(&maps[0], b, d.rows, d.n, d.ldb, 1, 0, 64, m_wide));
+            MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, 64, p.n_wide ? n_box / 64 : 0));
         } else {
             const long long b_rows = d.trans_b ? d.n : d.k;
             const int b_cols = d.trans_b ? d.k : d.n;
-            MFB_TRY(encode_16bit(&maps[0], b, b_rows, b_cols, d.ldb, shared ? 1 : d.groups, d.stride, m_mn ? 64 : 128));
-            MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, e.nt / e.cg));
+            MFB_TRY(encode_16bit(&maps[0], b, b_rows, b_cols, d.ldb, shared ? 1 : d.groups, d.stride, m_mn ? 64 : 128, m_wide));
+            MFB_TRY(encode_16bit(&maps[1], a, d.rows, d.k, d.lda, 1, 0, n_box));
             MFB_TRY(encode_16bit(&maps[2], a, d.rows, d.k, d.lda, 1, 0, 32));
             MFB_TRY(encode_16bit(&maps[3], a, d.rows, d.k, d.lda, 1, 0, 16));
         }

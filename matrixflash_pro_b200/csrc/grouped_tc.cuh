@@ -11,8 +11,8 @@
 // group), and its roles walk the same tile sequence, dealt out round-robin to the persistent workers.
 //
 // 16-bit operands whose rows TMA can address come by TMA, 64 of the contraction deep, 128-byte swizzle
-// (K-major tiles one box, or boxes of 32 and 16 rows; MN-major tiles boxes of 64 columns). All others (FP32, odd
-// strides) come by eight loader warps that read global memory into registers and write the same layout:
+// (K-major tiles a box of rows, MN-major tiles boxes of 64 columns). All others (FP32, odd
+// strides) come by loader warps that read global memory into registers and write the same layout:
 // 16-bit values as they are, FP32 as PLANES BF16 terms x = h + m + l (h cut, m and l rounded; exact with
 // three). Products hh, hm, mh, mm, hl, lh are kept (six MMAs per step, 1/6 of the BF16 rate); what is left
 // out is below 2^-21 of |a b|. Two terms (TF32 precision) keep hh, hm, mh.
@@ -47,6 +47,7 @@ struct GroupedParams {
     long long m_ld, m_stride, n_ld;  // bytes
     int m_align, n_align;
     int m_shared;  // all groups share one matrix: the tensor map has one
+    int m_wide, n_wide;  // MN-major operands whose rows are whole 64-column boxes: one copy brings all boxes of a slab
 };
 
 // KS = 64-deep slabs per stage. A stage has a fixed cost of a few hundred cycles (barrier wait, commit) beside its
@@ -67,13 +68,21 @@ struct GroupedConfig {
     static constexpr int kBarriers = STAGES * kStage;
     static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 6) + 8;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
-    static constexpr int kLoaders = TMA ? 2 : 8;  // warps; TMA: one per operand
+    // Warps. TMA: one producer per operand. Else 16 loader warps (odd strides: many small loads), or 8 (FP32: its six
+    // MMAs per step leave them time); roles are whole warpgroups then and share out the registers anew, for the
+    // epilogue's FP32 sums (in all no more than the launch has).
+    static constexpr int kLoaders = TMA ? 2 : PLANES == 1 ? 16 : 8;
     static constexpr int kMmaWarp = kLoaders, kFixWarp = kLoaders + 1;
-    static constexpr int kEpiWarp0 = TMA && RIGHT ? kLoaders + 2 : kLoaders + 1;
+    static constexpr int kEpiWarp0 = !TMA ? kLoaders + 4 : RIGHT ? kLoaders + 2 : kLoaders + 1;
+    static constexpr int kLoaderRegs = 64, kMmaRegs = PLANES == 1 ? 40 : 32, kEpiRegs = PLANES == 1 ? 104 : 160;
+    static constexpr int kLaunchRegs = PLANES == 1 ? 72 : 96;  // what the launch bounds leave a thread
+    static_assert(TMA || 32 * (kLoaders * kLoaderRegs + 4 * kMmaRegs + 8 * kEpiRegs) <= 32 * (kLoaders + 12) * kLaunchRegs,
+                  "register shares");
     static constexpr int kEpiWarps = 8;
     static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
     static constexpr int kTmemCols = 2 * NT;
-    static constexpr int kGranule = 16 * CG;  // N of an MMA is a multiple of this
+    // N of an MMA is a multiple of this: whole 64-column boxes per CTA where the N side is MN-major.
+    static constexpr int kGranule = (RIGHT ? 64 : 16) * CG;
     // Arrivals that complete a filled stage, besides the bytes of TMA copies: the loader warps', and in the leader of
     // a pair one from the peer. (An arrival across the pair is slow, so the peer's idle MMA warp makes it.)
     __device__ static int full_count(bool leader) { return TMA ? 1 : kLoaders + (CG == 2 && leader ? 1 : 0); }
@@ -255,8 +264,7 @@ struct GroupedChunk {
 };
 
 // One operand's 64-deep slabs on the way from global memory through registers into shared memory: WIDTH rows of the
-// tile (columns, where the operand is MN-major). A thread's chunks are 32 rows apart (K-major: 8 chunks a row) or
-// 256 / (WIDTH / 8) rows of the contraction (MN-major).
+// tile (columns, where the operand is MN-major). K-major rows have 8 chunks of eight elements, MN-major ones WIDTH / 8.
 template <class Cfg, int WIDTH, bool MN>
 struct GroupedSide {
     static constexpr int ES = Cfg::ES, kThreads = 32 * Cfg::kLoaders;
@@ -441,7 +449,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             bool ok = true;
             while (ok && work.next(t)) {
                 const int half = t.cols / CG;  // N-side rows of this CTA
-                const int n_rows = Cfg::N_MN ? (half + 63) / 64 * 64 : half;
+                // A copy costs the issuing thread more than a few rows too many cost the memory: one box, larger than
+                // needed, instead of several.
+                const int n_rows = Cfg::N_MN ? (p.n_wide ? Cfg::NTC : half)
+                                             : half > 32 ? Cfg::NTC : half > 16 ? 32 : 16;
                 const uint32_t bytes = Cfg::kMPlane + n_rows * 128;
                 const int f = t.f0 + 128 * rank, r = t.r0 + half * rank;
                 for (int kb = 0; kb < t.kb; ++kb, ++it) {
@@ -463,26 +474,30 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         if (CG == 2) tma_load_3d_pair(dst, map, to, x, y, z);
                         else tma_load_3d(dst, map, bar, x, y, z);
                     };
+                    auto load_wide = [&](uint8_t* dst, const CUtensorMap* map, int column, int y, int z) {
+                        if (CG == 2) tma_load_4d_pair(dst, map, to, 0, y, column / 64, z);
+                        else tma_load_4d(dst, map, bar, 0, y, column / 64, z);
+                    };
                     const int z = Cfg::RIGHT || p.m_shared ? 0 : t.e;
                     for (int j = 0; j < slabs; ++j) {
                         uint8_t* m_tile = smem + s * Cfg::kStage + j * Cfg::kSlab;
                         uint8_t* n_tile = m_tile + Cfg::kMBytes;
                         const int d0 = (Cfg::RIGHT ? t.t0 : 0) + (kb * Cfg::KS + j) * kGroupedDepth;
                         if (warp == 0) {
-                            if (Cfg::M_MN) {
+                            if (!Cfg::M_MN) {
+                                load(m_tile, &map_m, d0, f, z);
+                            } else if (p.m_wide) {
+                                load_wide(m_tile, &map_m, f, d0, z);
+                            } else {
                                 load(m_tile, &map_m, f, d0, z);
                                 load(m_tile + 8192, &map_m, f + 64, d0, z);
-                            } else {
-                                load(m_tile, &map_m, d0, f, z);
                             }
-                        } else if (Cfg::N_MN) {
-                            for (int b = 0; b < n_rows / 64; ++b) load(n_tile + b * 8192, &map_n, r + 64 * b, d0, 0);
-                        } else if (half == Cfg::NTC) {
-                            load(n_tile, &map_n, d0, r, 0);
+                        } else if (!Cfg::N_MN) {
+                            load(n_tile, half > 32 ? &map_n : half > 16 ? &map_n32 : &map_n16, d0, r, 0);
+                        } else if (p.n_wide) {
+                            load_wide(n_tile, &map_n, r, d0, 0);
                         } else {
-                            int row = 0;
-                            for (; row + 32 <= half; row += 32) load(n_tile + row * 128, &map_n32, d0, r + row, 0);
-                            if (row < half) load(n_tile + row * 128, &map_n16, d0, r + row, 0);
+                            for (int b = 0; b < n_rows / 64; ++b) load(n_tile + b * 8192, &map_n, r + 64 * b, d0, 0);
                         }
                     }
                 }
@@ -500,6 +515,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         // A slab's chunks of eight elements are dealt out to the threads; each keeps the next slab's in registers while
         // it writes this one's. Where a slab lies inside the operand (all but edges) a chunk costs a pointer step and
         // its loads.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kLoaderRegs));
         using M = GroupedSide<Cfg, 128, Cfg::M_MN>;
         using N = GroupedSide<Cfg, Cfg::NTC, Cfg::N_MN>;
         M m;
@@ -514,7 +530,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             n.start(p.n_base, p.n_ld, p.n_align, t.r0 + half * rank, half, Cfg::RIGHT ? p.k : t.t1, d0, d1, id);
             if (t.kb > 0) {
                 m.load(id);
-                n.load(id);
+                if (PLANES == 1) n.load(id);
             }
             for (int kb = 0; kb < t.kb; ++kb, ++it) {
                 const int s = it % STAGES;
@@ -526,15 +542,21 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 }
                 const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
                 m.store(m_tile, id);
-                if (kb + 1 < t.kb) m.load(id);
+                if (PLANES > 1) n.load(id);  // in the registers that M's chunks leave
                 n.store(m_tile + Cfg::kMBytes, id);
-                if (kb + 1 < t.kb) n.load(id);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full_bar[s]);
+                if (kb + 1 < t.kb) {
+                    m.load(id);
+                    if (PLANES == 1) n.load(id);
+                }
             }
         }
+    } else if (!Cfg::TMA && warp > Cfg::kMmaWarp && warp < Cfg::kEpiWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kMmaRegs));  // the rest of the MMA's warpgroup
     } else if (!Cfg::TMA && CG == 2 && warp == Cfg::kMmaWarp && !leader) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kMmaRegs));
         // ------------------------------------------------------------ tells the leader of the peer's filled stages
         if (lane == 0) {
             int it = 0;
@@ -553,6 +575,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (warp == Cfg::kMmaWarp) {
         // ------------------------------------------------------------ MMA issuer (leader)
+        if (!Cfg::TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kMmaRegs));
         if (lane == 0 && leader) {
             int it = 0, buf = 0;
             bool ok = true;
@@ -561,7 +584,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     umma_idesc_f16(Cfg::BM, t.cols, Cfg::M_MN, Cfg::N_MN, PLANES > 1 ? 1 : p.bf16);
                 uint32_t d_tmem = 0, acc = 0;
                 for (int kb = 0; kb < t.kb; ++kb, ++it) {
-                    if (kb == 0 || PLANES == 3) {
+                    if (PLANES == 3 || kb == 0) {
                         const int b = buf & 1;
                         if (!mbar_wait_bounded(&acc_empty_bar[b], ((buf >> 1) & 1) ^ 1, limit, abort_flag)) {
                             give_up(kStatusTimeoutMma);
@@ -584,31 +607,30 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         // 16-deep steps of this slab that the contraction still has
                         const int steps = min(kGroupedDepth / 16, t.steps - (kb * Cfg::KS + j) * (kGroupedDepth / 16));
                         const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage + j * Cfg::kSlab);
-                        const uint32_t n_addr = m_addr + Cfg::kMBytes;
-                        auto m_desc = [&](int pl, int ks) {
-                            const uint32_t a = m_addr + pl * Cfg::kMPlane;
-                            return Cfg::M_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
-                                             : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
-                        };
-                        auto n_desc = [&](int pl, int ks) {
-                            const uint32_t a = n_addr + pl * Cfg::kNPlane;
-                            return Cfg::N_MN ? umma_smem_desc(a + ks * 2048, 8192, 1024, kLayoutSwizzle128B)
-                                             : umma_smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B);
-                        };
-                        auto mma = [&](int mp, int np, int ks) {
-                            if (CG == 2) umma_f16_pair(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
-                            else umma_f16(d_tmem, m_desc(mp, ks), n_desc(np, ks), idesc, acc);
+                        const uint64_t m_desc = umma_smem_desc(m_addr, Cfg::M_MN ? 8192 : 16, 1024, kLayoutSwizzle128B);
+                        const uint64_t n_desc =
+                            umma_smem_desc(m_addr + Cfg::kMBytes, Cfg::N_MN ? 8192 : 16, 1024, kLayoutSwizzle128B);
+                        const uint32_t m_lo = static_cast<uint32_t>(m_desc), m_hi = static_cast<uint32_t>(m_desc >> 32);
+                        const uint32_t n_lo = static_cast<uint32_t>(n_desc), n_hi = static_cast<uint32_t>(n_desc >> 32);
+                        auto mma = [&](int mp, int np, int ks) {  // descriptors count 16-byte units
+                            umma_f16<CG>(d_tmem, m_lo + (mp * Cfg::kMPlane + ks * (Cfg::M_MN ? 2048 : 32)) / 16, m_hi,
+                                         n_lo + (np * Cfg::kNPlane + ks * (Cfg::N_MN ? 2048 : 32)) / 16, n_hi, idesc, acc);
                             acc = 1;
                         };
                         // The small products of all steps first: every addition truncates relative to what the
                         // accumulator holds, so only the last four cut at the sum's own size.
                         constexpr int kTerms = PLANES == 3 ? 6 : PLANES == 2 ? 3 : 1;
                         constexpr int kMTerm[6] = {2, 0, 1, 1, 0, 0}, kNTerm[6] = {0, 2, 1, 0, 1, 0};
+                        if (steps == kGroupedDepth / 16) {
 #pragma unroll
-                        for (int i = 6 - kTerms; i < 6; ++i)
+                            for (int i = 6 - kTerms; i < 6; ++i)
 #pragma unroll
-                            for (int ks = 0; ks < kGroupedDepth / 16; ++ks)
-                                if (ks < steps) mma(kMTerm[i], kNTerm[i], ks);
+                                for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                        } else {
+#pragma unroll
+                            for (int i = 6 - kTerms; i < 6; ++i)
+                                for (int ks = 0; ks < steps; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                        }
                     }
                     if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
                     else umma_commit(&empty_bar[s]);
@@ -643,7 +665,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             }
             phases ^= 1u << s;
             const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage + (t.slabs - 1) % Cfg::KS * Cfg::kSlab);
-            const int boxes = (t.cols / CG + 63) / 64;
+            const int boxes = t.cols / CG / 64;
             for (int b = 0; b < 2 + boxes; ++b) {
                 const uint32_t box = m_tile + (b < 2 ? b * 8192 : Cfg::kMBytes + (b - 2) * 8192);
                 for (int at = valid * 128 + lane * 16; at < end * 128; at += 512) GroupedChunk<2>::st(box + at, 0, 0, 0, 0);
@@ -667,6 +689,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (warp >= Cfg::kEpiWarp0) {
         // ------------------------------------------------------------ epilogue
+        if (!Cfg::TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kEpiRegs));
         const int quarter = warp & 3;                    // TMEM lanes of this warp
         const int part = (warp - Cfg::kEpiWarp0) >> 2;   // which of every two 16-column chunks
         const uint32_t acc_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
