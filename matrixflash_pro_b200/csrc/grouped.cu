@@ -13,6 +13,11 @@ namespace {
 
 int dtype_bytes(int dtype) { return dtype == MFB_DTYPE_F32 ? 4 : 2; }
 
+// Bytes from the first to behind the last element of `count` matrices of r rows.
+long long extent(long long r, long long ld, long long cols, long long count, long long stride, int bytes) {
+    return r == 0 || count == 0 ? 0 : ((r - 1) * ld + cols + (count - 1) * stride) * bytes;
+}
+
 // Checks that both entry points share. `right`: the gradient by the groups' matrices.
 mfb_status_t validate_grouped(const mfb_grouped_desc* d, const int* offsets, const void* a, const void* b,
                               const void* c, bool right) {
@@ -48,9 +53,6 @@ mfb_status_t validate_grouped(const mfb_grouped_desc* d, const int* offsets, con
     const bool reads = d->rows > 0 && d->k > 0 && d->groups > 0;
     if (!reads) return MFB_OK;
     if (!a || !b) return fail(MFB_EINVAL, "null A or B pointer");
-    auto extent = [](long long r, long long ld, long long cols, long long count, long long stride, int bytes) {
-        return r == 0 ? 0ll : ((r - 1) * ld + cols + (count - 1) * stride) * bytes;
-    };
     const char* cs = static_cast<const char*>(c);
     const char* as = static_cast<const char*>(a);
     const char* bs = static_cast<const char*>(b);

@@ -27,6 +27,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace mfb {
 
 constexpr int kGroupedMaxGroups = 1024;
@@ -68,16 +70,14 @@ struct GroupedConfig {
     static constexpr int kBarriers = STAGES * kStage;
     static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 6) + 8;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
-    // Warps. TMA: one producer per operand. Else 16 loader warps (odd strides: many small loads), or 8 (FP32: its six
-    // MMAs per step leave them time); roles are whole warpgroups then and share out the registers anew, for the
-    // epilogue's FP32 sums (in all no more than the launch has).
-    static constexpr int kLoaders = TMA ? 2 : PLANES == 1 ? 16 : 8;
+    // Warps. TMA: one producer per operand. Else 16 loader warps, since turning FP32 into three terms (or reading odd
+    // strides) takes many instructions; roles are whole warpgroups then and share out the registers anew, for the
+    // epilogue's FP32 sums (in all no more than the launch has: 896 threads of 72).
+    static constexpr int kLoaders = TMA ? 2 : 16;
     static constexpr int kMmaWarp = kLoaders, kFixWarp = kLoaders + 1;
     static constexpr int kEpiWarp0 = !TMA ? kLoaders + 4 : RIGHT ? kLoaders + 2 : kLoaders + 1;
-    static constexpr int kLoaderRegs = 64, kMmaRegs = PLANES == 1 ? 40 : 32, kEpiRegs = PLANES == 1 ? 104 : 160;
-    static constexpr int kLaunchRegs = PLANES == 1 ? 72 : 96;  // what the launch bounds leave a thread
-    static_assert(TMA || 32 * (kLoaders * kLoaderRegs + 4 * kMmaRegs + 8 * kEpiRegs) <= 32 * (kLoaders + 12) * kLaunchRegs,
-                  "register shares");
+    static constexpr int kLoaderRegs = 56, kMmaRegs = 72, kEpiRegs = 104;
+    static_assert(512 * kLoaderRegs + 128 * kMmaRegs + 256 * kEpiRegs <= 896 * 72, "register shares");
     static constexpr int kEpiWarps = 8;
     static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
     static constexpr int kTmemCols = 2 * NT;
@@ -172,7 +172,7 @@ __device__ __forceinline__ void grouped_store16(const GroupedParams& p, long lon
     }
 }
 
-// Eight consecutive elements of a row in global memory.
+// Eight consecutive FP32 elements of a row in global memory.
 template <int ES>
 struct GroupedChunk {
     uint32_t w[2 * ES];  // ES 2: four words of two values; ES 4: eight FP32 values
@@ -184,33 +184,21 @@ struct GroupedChunk {
 
     // All eight are there; `align`: bytes that the address is a multiple of.
     __device__ __forceinline__ void load(const char* src, int align) {
-        if (align >= 16) {
-            if (ES == 4 && align >= 32) {
-                asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4 % (2 * ES)]), "=r"(w[5 % (2 * ES)]),
-                               "=r"(w[6 % (2 * ES)]), "=r"(w[7 % (2 * ES)])
-                             : "l"(src));
-                return;
-            }
+        constexpr int kWords = 2 * ES;
+        if (ES == 4 && align >= 32) {
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4 % kWords]), "=r"(w[5 % kWords]),
+                           "=r"(w[6 % kWords]), "=r"(w[7 % kWords])
+                         : "l"(src));
+        } else if (align >= 16) {
 #pragma unroll
-            for (int i = 0; i < ES / 2; ++i) {
+            for (int i = 0; i < kWords / 4; ++i) {
                 const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
                 w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
-        } else if (ES == 4 || align >= 4) {
-#pragma unroll
-            for (int i = 0; i < 2 * ES; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
         } else {
-            // Rows start at any even address: the aligned words between the first and the last value.
-            const bool odd = reinterpret_cast<uintptr_t>(src) & 2;
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(src + (odd ? 2 : 0));
-            const uint32_t edge = __ldg(reinterpret_cast<const uint16_t*>(src) + (odd ? 0 : 6));
-            const uint32_t last = __ldg(reinterpret_cast<const uint16_t*>(src) + 7);
-            const uint32_t v0 = __ldg(words), v1 = __ldg(words + 1), v2 = __ldg(words + 2);
-            w[0] = odd ? edge | v0 << 16 : v0;
-            w[1] = odd ? __funnelshift_r(v0, v1, 16) : v1;
-            w[2] = odd ? __funnelshift_r(v1, v2, 16) : v2;
-            w[3] = odd ? v2 >> 16 | last << 16 : edge | last << 16;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
         }
     }
 
@@ -226,13 +214,8 @@ struct GroupedChunk {
         }
         const int count = cols - col;
 #pragma unroll
-        for (int i = 0; i < 7; ++i) {
-            if (i >= count) continue;
-            if (ES == 2)
-                w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + i)) << (16 * (i % 2));
-            else
-                w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
-        }
+        for (int i = 0; i < 7; ++i)
+            if (i < count) w[i % (2 * ES)] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
     }
 
     // Into 16 bytes of each plane at shared address `to`.
@@ -273,61 +256,134 @@ struct GroupedSide {
     static constexpr int kApart = kThreads / kPerRow;  // rows between a thread's chunks
     static constexpr int kPlane = WIDTH * 128;
     GroupedChunk<ES> c[kChunks];
-    const char* base;
     const char* at[MN ? 1 : kChunks];  // this thread's chunks of the next slab
-    long long ld;
-    int align, first, width, last, d0, d1;
-    bool inside;
 
-    // Rows (columns) [first_, first_ + width_) of the operand, which ends at last_; contraction [d0_, d1_).
-    __device__ __forceinline__ void start(const char* base_, long long ld_, int align_, int first_, int width_, int last_,
-                                          int d0_, int d1_, int id) {
-        base = base_, ld = ld_, align = align_, first = first_, width = width_, last = last_, d0 = d0_, d1 = d1_;
-        inside = MN ? first + WIDTH <= last : first < last;
+    // The tile's place in the operand: rows (columns) [first, first + width), which the operand has up to last. Put
+    // together where it is used, from the kernel's parameters and the tile, to leave the registers to the chunks.
+    struct Place {
+        const char* base;
+        long long ld;
+        int align, first, width, last;
+
+        __device__ __forceinline__ bool inside() const { return MN ? first + WIDTH <= last : first < last; }
+    };
+
+    // The contraction starts at d0.
+    __device__ __forceinline__ void start(const Place& o, int d0, int id) {
         if (MN) {
-            at[0] = base + (d0 + id / kPerRow) * ld + static_cast<long long>(first + id % kPerRow * 8) * ES;
+            at[0] = o.base + (d0 + id / kPerRow) * o.ld + static_cast<long long>(o.first + id % kPerRow * 8) * ES;
         } else {
 #pragma unroll
             for (int i = 0; i < (MN ? 1 : kChunks); ++i)  // rows past the end repeat the last: their results go nowhere
-                at[i] = base + min(first + i * kApart + id / 8, last - 1) * ld + static_cast<long long>(d0 + id % 8 * 8) * ES;
+                at[i] = o.base + min(o.first + i * kApart + id / 8, o.last - 1) * o.ld +
+                        static_cast<long long>(d0 + id % 8 * 8) * ES;
         }
     }
 
-    __device__ __forceinline__ bool has(int i, int id) const {  // whether chunk i is one of the tile's
+    __device__ __forceinline__ static bool has(int i, int id) {  // whether chunk i is one of the tile's
         return (WIDTH * 8) % kThreads == 0 || i * kThreads + id < WIDTH * 8;
     }
 
-    __device__ __forceinline__ void load(int id) {
-        if (inside && d0 + kGroupedDepth <= d1) {
+    // The slab from d0 on of a contraction that ends at d1.
+    __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id) {
+        if (o.inside() && d0 + kGroupedDepth <= d1) {
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 if (!has(i, id)) continue;
                 if (MN) {
-                    c[i].load(at[0] + i * kApart * ld, align);
-                } else if (i * kApart < width) {
-                    c[i].load(at[i], align);
+                    c[i].load(at[0] + i * kApart * o.ld, o.align);
+                } else if (i * kApart < o.width) {
+                    c[i].load(at[i], o.align);
                     at[i] += kGroupedDepth * ES;
                 }
             }
-            if (MN) at[0] += kGroupedDepth * ld;
+            if (MN) at[0] += kGroupedDepth * o.ld;
         } else {
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 if (!has(i, id)) continue;
                 const int row = i * kApart + id / kPerRow, col = id % kPerRow * 8;
-                if (MN) c[i].load_some(base, ld, align, d0 + row, d1, first + col, last);
-                else c[i].load_some(base, ld, align, first + row, last, d0 + col, d1);
+                if (MN) c[i].load_some(o.base, o.ld, o.align, d0 + row, d1, o.first + col, o.last);
+                else c[i].load_some(o.base, o.ld, o.align, o.first + row, o.last, d0 + col, d1);
             }
         }
-        d0 += kGroupedDepth;
     }
 
-    __device__ __forceinline__ void store(uint32_t tile, int id) const {
+    __device__ __forceinline__ void store(uint32_t tile, int width, int id) const {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             if (!has(i, id) || (!MN && i * kApart >= width)) continue;
             const int row = i * kApart + id / kPerRow, col = id % kPerRow, box = MN ? col / 8 : 0;
             c[i].template store<Cfg::PLANES>(tile + box * 8192 + row * 128 + (((col % 8) ^ (row & 7)) << 4), kPlane);
+        }
+    }
+};
+
+// The same for 16-bit operands that TMA cannot address, whose rows start at any even address: a warp takes 64 elements
+// of a row at a time, a word per lane, so that a load touches one or two lines however the row lies. A warp's segments
+// are a multiple of eight rows apart, so they all start on a word or all between words; then lanes pass halves on to
+// their neighbours, and the first half of each segment comes by one load for all of them.
+template <class Cfg, int WIDTH, bool MN>
+struct GroupedSide16 {
+    static constexpr int kWarps = Cfg::TMA ? 16 : Cfg::kLoaders;  // (TMA kernels do not use it)
+    static constexpr int kSegments = WIDTH / kWarps;              // of 64 elements, per warp
+    static constexpr int kBoxes = MN ? WIDTH / 64 : 1;
+    static constexpr int kApart = kWarps / kBoxes;  // rows between a warp's segments
+    static_assert(WIDTH % kWarps == 0 && kSegments <= 32 && kApart % 8 == 0, "segments");
+    using Place = typename GroupedSide<Cfg, WIDTH, MN>::Place;
+    uint32_t w[kSegments];
+    uint32_t edge;   // lane i: element 0 of segment i
+    const char* at;  // segment 0 of the next slab
+    bool shifted;    // what is in w starts between words
+
+    __device__ __forceinline__ void start(const Place& o, int d0, int id) {
+        const int warp = id / 32;
+        const int row = MN ? d0 + warp / kBoxes : o.first + warp, col = MN ? o.first + warp % kBoxes * 64 : d0;
+        at = o.base + row * o.ld + static_cast<long long>(col) * 2;
+    }
+
+    __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id) {
+        const int lane = id % 32, warp = id / 32;
+        const long long step = kApart * o.ld;
+        // One element more than the segments have: a lane's word may end behind them.
+        if (MN ? o.first + WIDTH < o.last && d0 + kGroupedDepth <= d1 : d0 + kGroupedDepth < d1) {
+            const uint32_t between = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at)) & 2u;
+            shifted = between != 0;
+            if (lane < kSegments && (MN || o.first + warp + lane * kApart < o.last))
+                edge = __ldg(reinterpret_cast<const uint16_t*>(at + lane * step));
+            const char* src = at + between + lane * 4;
+#pragma unroll
+            for (int i = 0; i < kSegments; ++i, src += step)
+                if (MN || o.first + warp + i * kApart < o.last) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src));
+        } else {
+            shifted = false;
+            const int col = (MN ? o.first + warp % kBoxes * 64 : d0) + 2 * lane, cols = MN ? o.last : d1;
+            const uint16_t* src = reinterpret_cast<const uint16_t*>(at) + 2 * lane;
+            int row = MN ? d0 + warp / kBoxes : o.first + warp;
+            const int rows = MN ? d1 : o.last;
+#pragma unroll
+            for (int i = 0; i < kSegments; ++i, row += kApart, src += step / 2) {
+                w[i] = 0;
+                if (row < rows && col < cols) w[i] = __ldg(src);
+                if (row < rows && col + 1 < cols) w[i] |= static_cast<uint32_t>(__ldg(src + 1)) << 16;
+            }
+        }
+        at += MN ? kGroupedDepth * o.ld : kGroupedDepth * 2;
+    }
+
+    // Rows past the operand's end hold what they held: their results go nowhere.
+    __device__ __forceinline__ void store(uint32_t tile, int width, int id) const {
+        const int lane = id % 32, warp = id / 32, row = warp / kBoxes;
+        const uint32_t to = tile + warp % kBoxes * 8192 + row * 128 + (((lane / 4) ^ (row & 7)) << 4) + lane % 4 * 4;
+#pragma unroll
+        for (int i = 0; i < kSegments; ++i) {
+            if (!MN && warp + i * kApart >= width) continue;
+            uint32_t v = w[i];
+            if (shifted) {
+                const uint32_t before = __shfl_up_sync(~0u, v, 1), first = __shfl_sync(~0u, edge, i);
+                v = (lane ? before >> 16 : first) | v << 16;
+            }
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i * kApart * 128), "r"(v) : "memory");
         }
     }
 };
@@ -516,8 +572,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         // it writes this one's. Where a slab lies inside the operand (all but edges) a chunk costs a pointer step and
         // its loads.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kLoaderRegs));
-        using M = GroupedSide<Cfg, 128, Cfg::M_MN>;
-        using N = GroupedSide<Cfg, Cfg::NTC, Cfg::N_MN>;
+        using M = std::conditional_t<Cfg::ES == 2, GroupedSide16<Cfg, 128, Cfg::M_MN>, GroupedSide<Cfg, 128, Cfg::M_MN>>;
+        using N = std::conditional_t<Cfg::ES == 2, GroupedSide16<Cfg, Cfg::NTC, Cfg::N_MN>, GroupedSide<Cfg, Cfg::NTC, Cfg::N_MN>>;
         M m;
         N n;
         const int id = threadIdx.x;
@@ -526,11 +582,18 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         while (ok && work.next(t)) {
             const int half = t.cols / CG;
             const int d0 = Cfg::RIGHT ? t.t0 : 0, d1 = Cfg::RIGHT ? t.t1 : p.k;
-            m.start(p.m_base + (Cfg::RIGHT ? 0 : t.e * p.m_stride), p.m_ld, p.m_align, t.f0 + 128 * rank, 128, p.n, d0, d1, id);
-            n.start(p.n_base, p.n_ld, p.n_align, t.r0 + half * rank, half, Cfg::RIGHT ? p.k : t.t1, d0, d1, id);
+            auto m_place = [&] {
+                return typename M::Place{p.m_base + (Cfg::RIGHT ? 0 : t.e * p.m_stride), p.m_ld, p.m_align, t.f0 + 128 * rank,
+                                         128, p.n};
+            };
+            auto n_place = [&] {
+                return typename N::Place{p.n_base, p.n_ld, p.n_align, t.r0 + half * rank, half, Cfg::RIGHT ? p.k : t.t1};
+            };
+            m.start(m_place(), d0, id);
+            n.start(n_place(), d0, id);
             if (t.kb > 0) {
-                m.load(id);
-                if (PLANES == 1) n.load(id);
+                m.load(m_place(), d0, d1, id);
+                n.load(n_place(), d0, d1, id);
             }
             for (int kb = 0; kb < t.kb; ++kb, ++it) {
                 const int s = it % STAGES;
@@ -541,15 +604,14 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     break;
                 }
                 const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
-                m.store(m_tile, id);
-                if (PLANES > 1) n.load(id);  // in the registers that M's chunks leave
-                n.store(m_tile + Cfg::kMBytes, id);
+                m.store(m_tile, 128, id);
+                n.store(m_tile + Cfg::kMBytes, half, id);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full_bar[s]);
                 if (kb + 1 < t.kb) {
-                    m.load(id);
-                    if (PLANES == 1) n.load(id);
+                    m.load(m_place(), d0 + (kb + 1) * kGroupedDepth, d1, id);
+                    n.load(n_place(), d0 + (kb + 1) * kGroupedDepth, d1, id);
                 }
             }
         }
