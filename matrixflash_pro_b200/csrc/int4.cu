@@ -41,9 +41,9 @@ struct Int4Params {
 // ------------------------------------------------------------------------------------
 // Quantising
 // ------------------------------------------------------------------------------------
-// The integer nearest to w / s, ties to even, |result| <= 64. The FP32 quotient decides except next to a
-// border between two codes, where the remainder w - q s does: it is exact in FP32 there, since w and q s
-// agree to within s.
+// The integer nearest to w / s, ties to even, |result| <= 64. The FP32
+// quotient decides except next to a border, where the remainder w - q s does: it is exact in FP32 there, since w and
+// q s agree to within s.
 __device__ __forceinline__ float nearest_code(float w, float s, float inv) {
     const float t = fminf(fmaxf(w * inv, -64.0f), 64.0f);
     float q = rintf(t);
@@ -71,26 +71,45 @@ __device__ __forceinline__ __nv_bfloat16 saturated_scale<__nv_bfloat16>(double s
     return __float2bfloat16_rn(static_cast<float>(fmin(s, 3.3895313892515355e38)));
 }
 
-// One warp per row and group.
-template <typename T, typename TS>
-__global__ void __launch_bounds__(256) quantize_int4_kernel(const Int4Params p, const T* __restrict__ w,
-                                                            long long ldw, long long stride_w) {
-    const long long unit = (blockIdx.x * 256ll + threadIdx.x) / 32;
-    const int lane = threadIdx.x % 32;
-    if (unit >= p.rows * p.groups) return;
-    const long long row = unit / p.groups;
-    const int g = static_cast<int>(unit - row * p.groups);
-    const T* src = w + (row / p.n) * stride_w + (row % p.n) * ldw;
-    const int per = p.group / 32;  // 1, 2 or 4 consecutive columns per lane
-    const int j0 = g * p.group + lane * per;
-    float v[4];
-    float lo = 0.0f, hi = 0.0f;
-    for (int i = 0; i < per; ++i) {
-        v[i] = j0 + i < p.k ? to_f32(src[j0 + i]) : 0.0f;
-        lo = fminf(lo, v[i]);
-        hi = fmaxf(hi, v[i]);
+// Sixteen elements and eight bytes of codes per lane (the bytes of one lane's codes are a whole word or two), so two,
+// four or eight lanes to a group, and one division in double precision for a warp's 16, 8 or 4 groups. Bound by
+// memory (read once, a quarter or an eighth written) with about 15 instructions an element in front of it; a warp per
+// group, as a first version had it, spent most of its time on the division and on stores of single bytes.
+// vec: rows of w that start on 16 bytes.
+template <typename T, typename TS, int GROUP>
+__global__ void __launch_bounds__(256) quantize_int4_kernel(const Int4Params p, const T* __restrict__ w, long long ldw,
+                                                            long long stride_w, int cells, bool vec) {
+    constexpr int kEach = 16, kLanes = GROUP / kEach;
+    const long long unit = blockIdx.x * 256ll + threadIdx.x;  // a lane's 16 columns of a row; `cells` of them a row
+    const long long row = unit / cells;
+    const int j0 = static_cast<int>(unit - row * cells) * kEach;
+    const bool live = row < p.rows;
+    float v[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) v[i] = 0.0f;
+    if (live) {
+        const long long e = p.experts == 1 ? 0 : row / p.n;
+        const T* src = w + e * stride_w + (row - e * p.n) * ldw + j0;
+        if (vec && j0 + kEach <= p.k) {
+            constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+            for (int i = 0; i < kEach / kPer; ++i) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(src) + i);
+                const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[i * kPer + j] = to_f32(t[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (j0 + i < p.k) v[i] = to_f32(src[i]);
+        }
     }
-    for (int d = 16; d; d /= 2) {
+    float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]);
+#pragma unroll
+    for (int d = kLanes / 2; d; d /= 2) {
         lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
         hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
     }
@@ -100,37 +119,49 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const Int4Params p, 
     const float s = to_f32(scale), inv = 1.0f / s;
     float z = 8.0f;
     if (p.zeros) z = fminf(fmaxf(nearest_code(-lo, s, inv), 0.0f), 15.0f);
-    if (lane == 0) {
-        static_cast<TS*>(p.scales)[unit] = scale;
-        if (p.zeros) p.zeros[unit] = static_cast<unsigned char>(z);
+    if (!live) return;
+    if (threadIdx.x % kLanes == 0 && j0 < p.groups * GROUP) {
+        const long long at = row * p.groups + j0 / GROUP;
+        static_cast<TS*>(p.scales)[at] = scale;
+        if (p.zeros) p.zeros[at] = static_cast<unsigned char>(z);
     }
-    unsigned codes = 0;
-    for (int i = 0; i < per; ++i) {
+    if (j0 / 2 >= p.row_bytes) return;
+    uint32_t codes[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
         const float q = fminf(fmaxf(nearest_code(v[i], s, inv) + z, 0.0f), 15.0f);
-        codes |= static_cast<unsigned>(q) << (4 * i);
+        codes[i / 8] |= static_cast<uint32_t>(q) << (4 * (i % 8));
     }
-    if (per == 1) codes |= __shfl_down_sync(~0u, codes, 1) << 4;  // lanes pair up: two codes per byte
-    unsigned char* dst = p.packed + row * p.row_bytes;
-    if (per == 1 && (lane & 1)) return;
-    for (int i = 0; i < (per + 1) / 2; ++i)
-        if (j0 / 2 + i < p.row_bytes) dst[j0 / 2 + i] = static_cast<unsigned char>(codes >> (8 * i));
+    *reinterpret_cast<uint2*>(p.packed + row * p.row_bytes + j0 / 2) = make_uint2(codes[0], codes[1]);
 }
 
+// Sixteen columns of a row per lane: one load of codes, one scale, stores of 16 bytes where the rows allow it (vec).
 template <typename TS, typename T>
 __global__ void __launch_bounds__(256) dequantize_int4_kernel(const Int4Params p, T* __restrict__ out, long long ldo,
-                                                              long long stride_o) {
-    const long long total = p.rows * p.row_bytes;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const long long row = i / p.row_bytes;
-        const int j = 2 * static_cast<int>(i - row * p.row_bytes);
-        if (j >= p.k) continue;
-        const long long at = row * p.groups + j / p.group;
-        const float s = to_f32(static_cast<const TS*>(p.scales)[at]);
-        const float z = p.zeros ? static_cast<float>(p.zeros[at]) : 8.0f;
-        const unsigned b = p.packed[i];
-        T* dst = out + (row / p.n) * stride_o + (row % p.n) * ldo + j;
-        dst[0] = from_f32<T>((static_cast<float>(b & 15u) - z) * s);
-        if (j + 1 < p.k) dst[1] = from_f32<T>((static_cast<float>(b >> 4) - z) * s);
+                                                              long long stride_o, int cells, bool vec) {
+    constexpr int kEach = 16;
+    const long long unit = blockIdx.x * 256ll + threadIdx.x;
+    const long long row = unit / cells;
+    const int j0 = static_cast<int>(unit - row * cells) * kEach;
+    if (row >= p.rows || j0 >= p.k) return;
+    const uint2 codes = __ldg(reinterpret_cast<const uint2*>(p.packed + row * p.row_bytes + j0 / 2));
+    const long long at = row * p.groups + j0 / p.group;
+    const float s = to_f32(static_cast<const TS*>(p.scales)[at]);
+    const float z = p.zeros ? static_cast<float>(p.zeros[at]) : 8.0f;
+    const long long e = p.experts == 1 ? 0 : row / p.n;
+    T* dst = out + e * stride_o + (row - e * p.n) * ldo + j0;
+    alignas(16) T v[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        v[i] = from_f32<T>((static_cast<float>(((i < 8 ? codes.x : codes.y) >> (4 * (i % 8))) & 15u) - z) * s);
+    if (vec && j0 + kEach <= p.k) {
+#pragma unroll
+        for (int i = 0; i < kEach * static_cast<int>(sizeof(T)) / 16; ++i)
+            reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (j0 + i < p.k) dst[i] = v[i];
     }
 }
 
@@ -795,13 +826,20 @@ MFB_API mfb_status_t mfb_quantize_int4(int device, mfb_stream_t stream, const vo
     MFB_TRY(validate_rows(p, w, dtype, ldw, stride_w, false));
     DeviceGuard guard;
     MFB_TRY(select_device(device));
-    const long long blocks = (p.rows * p.groups + 7) / 8;
+    const int cells = p.groups * (p.group / 16);  // whole groups, so that a group's lanes are in one warp
+    const long long blocks = (p.rows * cells + 255) / 256;
     if (blocks > 0x7fffffffLL) return fail(MFB_EINVAL, "4-bit matrix has too many groups");
+    const long long size = dtype_bytes(dtype);
+    const bool vec = aligned16(w) && (p.n <= 1 || ldw * size % 16 == 0) && (p.experts == 1 || stride_w * size % 16 == 0);
     return with_dtype(dtype, [&](auto t) {
         return with_dtype(out->scale_dtype, [&](auto ts) {
             using T = decltype(t);
-            quantize_int4_kernel<T, decltype(ts)><<<static_cast<unsigned>(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-                p, static_cast<const T*>(w), ldw, stride_w);
+            using TS = decltype(ts);
+            const auto kernel = out->group == 32   ? &quantize_int4_kernel<T, TS, 32>
+                                : out->group == 64 ? &quantize_int4_kernel<T, TS, 64>
+                                                   : &quantize_int4_kernel<T, TS, 128>;
+            kernel<<<static_cast<unsigned>(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                p, static_cast<const T*>(w), ldw, stride_w, cells, vec);
             MFB_CUDA_TRY(cudaGetLastError(), "quantize_int4 launch");
             return MFB_OK;
         });
@@ -818,11 +856,16 @@ MFB_API mfb_status_t mfb_dequantize_int4(int device, mfb_stream_t stream, const 
     MFB_TRY(validate_rows(p, out, dtype, ldo, stride_o, true));
     DeviceGuard guard;
     MFB_TRY(select_device(device));
+    const int cells = p.row_bytes / 8;
+    const long long blocks = (p.rows * cells + 255) / 256;
+    if (blocks > 0x7fffffffLL) return fail(MFB_EINVAL, "4-bit matrix is too large");
+    const long long size = dtype_bytes(dtype);
+    const bool vec = aligned16(out) && (p.n <= 1 || ldo * size % 16 == 0) && (p.experts == 1 || stride_o * size % 16 == 0);
     return with_dtype(m->scale_dtype, [&](auto ts) {
         return with_dtype(dtype, [&](auto t) {
             using T = decltype(t);
-            dequantize_int4_kernel<decltype(ts), T><<<8 * current_sm_count(), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-                p, static_cast<T*>(out), ldo, stride_o);
+            dequantize_int4_kernel<decltype(ts), T><<<static_cast<unsigned>(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                p, static_cast<T*>(out), ldo, stride_o, cells, vec);
             MFB_CUDA_TRY(cudaGetLastError(), "dequantize_int4 launch");
             return MFB_OK;
         });
