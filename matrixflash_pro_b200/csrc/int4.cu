@@ -41,19 +41,39 @@ struct Int4Params {
 // ------------------------------------------------------------------------------------
 // Quantising
 // ------------------------------------------------------------------------------------
-// The integer nearest to w / s, ties to even, |result| <= 64. The FP32
-// quotient decides except next to a border, where the remainder w - q s does: it is exact in FP32 there, since w and
-// q s agree to within s.
-__device__ __forceinline__ float nearest_code(float w, float s, float inv) {
-    const float t = fminf(fmaxf(w * inv, -64.0f), 64.0f);
-    float q = rintf(t);
-    if (fabsf(t - q) > 0.499f) {
-        const float r = fmaf(-q, s, w);
-        const float half = 0.5f * s;
-        if (r > half || (r == half && (static_cast<int>(q) & 1))) q += 1.0f;
-        else if (r < -half || (r == -half && (static_cast<int>(q) & 1))) q -= 1.0f;
-    }
-    return q;
+// a / b; a 64-bit division only where a needs it (it takes four times as long as all else that a thread does).
+__device__ __forceinline__ long long quotient(long long a, int b) {
+    if (static_cast<unsigned long long>(a) >> 32) return a / b;
+    return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+}
+
+// The integer nearest to w / s, ties to even: the quotient of two FP32 numbers in double precision is never rounded
+// onto or across a border between two integers below 2^24.
+__device__ __noinline__ int exact_code(float w, float s) {
+    return static_cast<int>(rint(fmin(fmax(static_cast<double>(w) / s, -64.0), 64.0)));
+}
+
+// clamp(nearest integer to w / s + z, 0, 15), from inv = 1 / s in FP32. The integer that w inv gives may be the wrong
+// one next to a border between two; the remainder r = w - q s, exact in FP32, tells: q moves where r is above s / 2, or
+// is s / 2 and q odd (16-bit weights and scales meet such ties often: one in a few hundred). below = the FP32 number
+// under half = s / 2.
+constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits
+__device__ __forceinline__ int fast_code(float w, float s, float inv, float half, float below, int z) {
+    const float m = fmaf(w, inv, kRound);
+    const float r = fmaf(kRound - m, s, w);
+    int q = __float_as_int(m);
+    const float most = q & 1 ? below : half;
+    if (r > most) ++q;
+    if (r < -most) --q;
+    return __viaddmin_s32_relu(q, z - 0x4b400000, 15);
+}
+
+// x / divisor (15 or 7) rounded to double and then to FP32, x = hi - lo. Where x is an FP32 number, so is rounding the
+// quotient once: it is never within 2^-30 of the middle between two of them.
+__device__ __forceinline__ double scale_of(float hi, float lo, float divisor) {
+    const float x = hi - lo, back = x - hi;
+    if ((hi - (x - back)) + (-lo - back) == 0.0f) return __fdiv_rn(x, divisor);
+    return (static_cast<double>(hi) - lo) / divisor;
 }
 
 template <typename TS>
@@ -73,7 +93,7 @@ __device__ __forceinline__ __nv_bfloat16 saturated_scale<__nv_bfloat16>(double s
 
 // Sixteen elements and eight bytes of codes per lane (the bytes of one lane's codes are a whole word or two), so two,
 // four or eight lanes to a group, and one division in double precision for a warp's 16, 8 or 4 groups. Bound by
-// memory (read once, a quarter or an eighth written) with about 15 instructions an element in front of it; a warp per
+// memory (read once, a quarter or an eighth written), with about fifteen instructions an element before that; a warp per
 // group, as a first version had it, spent most of its time on the division and on stores of single bytes.
 // vec: rows of w that start on 16 bytes.
 template <typename T, typename TS, int GROUP>
@@ -81,14 +101,14 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const Int4Params p, 
                                                             long long stride_w, int cells, bool vec) {
     constexpr int kEach = 16, kLanes = GROUP / kEach;
     const long long unit = blockIdx.x * 256ll + threadIdx.x;  // a lane's 16 columns of a row; `cells` of them a row
-    const long long row = unit / cells;
+    const long long row = quotient(unit, cells);
     const int j0 = static_cast<int>(unit - row * cells) * kEach;
     const bool live = row < p.rows;
     float v[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) v[i] = 0.0f;
     if (live) {
-        const long long e = p.experts == 1 ? 0 : row / p.n;
+        const long long e = p.experts == 1 ? 0 : quotient(row, p.n);
         const T* src = w + e * stride_w + (row - e * p.n) * ldw + j0;
         if (vec && j0 + kEach <= p.k) {
             constexpr int kPer = 16 / sizeof(T);
@@ -113,12 +133,15 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const Int4Params p, 
         lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
         hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
     }
-    const double range = p.zeros ? (static_cast<double>(hi) - lo) / 15.0 : fmax(-static_cast<double>(lo), hi) / 7.0;
+    const double range = p.zeros ? scale_of(hi, lo, 15.0f) : scale_of(fmaxf(-lo, hi), 0.0f, 7.0f);
     TS scale = saturated_scale<TS>(range);
     if (to_f32(scale) == 0.0f) scale = from_f32<TS>(1.0f);
     const float s = to_f32(scale), inv = 1.0f / s;
-    float z = 8.0f;
-    if (p.zeros) z = fminf(fmaxf(nearest_code(-lo, s, inv), 0.0f), 15.0f);
+    // A saturated scale (quotients beyond the fast path's integers) or one without an FP32 reciprocal.
+    const bool odd = range > 2.0 * s || s < 1e-37f;
+    const float half = 0.5f * s, below = __int_as_float(__float_as_int(half) - 1);
+    int z = 8;
+    if (p.zeros) z = odd ? min(max(exact_code(-lo, s), 0), 15) : fast_code(-lo, s, inv, half, below, 0);
     if (!live) return;
     if (threadIdx.x % kLanes == 0 && j0 < p.groups * GROUP) {
         const long long at = row * p.groups + j0 / GROUP;
@@ -127,10 +150,14 @@ __global__ void __launch_bounds__(256) quantize_int4_kernel(const Int4Params p, 
     }
     if (j0 / 2 >= p.row_bytes) return;
     uint32_t codes[2] = {0, 0};
+    if (!odd) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const float q = fminf(fmaxf(nearest_code(v[i], s, inv) + z, 0.0f), 15.0f);
-        codes[i / 8] |= static_cast<uint32_t>(q) << (4 * (i % 8));
+        for (int i = 0; i < kEach; ++i)
+            codes[i / 8] |= static_cast<uint32_t>(fast_code(v[i], s, inv, half, below, z)) << (4 * (i % 8));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            codes[i / 8] |= static_cast<uint32_t>(min(max(exact_code(v[i], s) + z, 0), 15)) << (4 * (i % 8));
     }
     *reinterpret_cast<uint2*>(p.packed + row * p.row_bytes + j0 / 2) = make_uint2(codes[0], codes[1]);
 }
@@ -141,19 +168,19 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const Int4Params p
                                                               long long stride_o, int cells, bool vec) {
     constexpr int kEach = 16;
     const long long unit = blockIdx.x * 256ll + threadIdx.x;
-    const long long row = unit / cells;
+    const long long row = quotient(unit, cells);
     const int j0 = static_cast<int>(unit - row * cells) * kEach;
     if (row >= p.rows || j0 >= p.k) return;
     const uint2 codes = __ldg(reinterpret_cast<const uint2*>(p.packed + row * p.row_bytes + j0 / 2));
     const long long at = row * p.groups + j0 / p.group;
     const float s = to_f32(static_cast<const TS*>(p.scales)[at]);
-    const float z = p.zeros ? static_cast<float>(p.zeros[at]) : 8.0f;
-    const long long e = p.experts == 1 ? 0 : row / p.n;
+    const float z = 8388608.0f + (p.zeros ? static_cast<float>(p.zeros[at]) : 8.0f);
+    const long long e = p.experts == 1 ? 0 : quotient(row, p.n);
     T* dst = out + e * stride_o + (row - e * p.n) * ldo + j0;
     alignas(16) T v[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-        v[i] = from_f32<T>((static_cast<float>(((i < 8 ? codes.x : codes.y) >> (4 * (i % 8))) & 15u) - z) * s);
+        v[i] = from_f32<T>((__uint_as_float((((i < 8 ? codes.x : codes.y) >> (4 * (i % 8))) & 15u) | 0x4b000000u) - z) * s);  // 2^23 + q
     if (vec && j0 + kEach <= p.k) {
 #pragma unroll
         for (int i = 0; i < kEach * static_cast<int>(sizeof(T)) / 16; ++i)

@@ -103,6 +103,18 @@ def test_quantise_on_the_borders(symmetric):
         assert torch.isfinite(mf.dequantize_int4(m, F32)).all()
 
 
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_quantise_the_smallest_scales(symmetric):
+    """Weights near the end of FP32's range, where a scale has no reciprocal."""
+    w = _normal((40, 64), F32, 1) * torch.logspace(-44, -36, 40, device="cuda", dtype=torch.float64)[:, None]
+    w = w.to(F32)
+    m = mf.quantize_int4(w, 32, symmetric)
+    q, s, z = _quantised(w, 32, symmetric, F32)
+    mf.sync()
+    assert torch.equal(m.scales, s) and torch.equal(_unpack(m.packed, 64), q)
+    assert symmetric or torch.equal(m.zeros.long(), z)
+
+
 def test_quantise_strided_weights():
     whole = _normal((6, 40, 300), BF16, 1)
     for w in (whole[::2, 1:, 3:260], whole[:, ::3, :299], whole[1, :, 7:200], whole[:, :1, :64]):
