@@ -71,13 +71,15 @@ struct GroupedConfig {
     static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 6) + 8;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
     // Warps. TMA: one producer per operand. Else 16 loader warps, since turning FP32 into three terms (or reading odd
-    // strides) takes many instructions; roles are whole warpgroups then and share out the registers anew, for the
-    // epilogue's FP32 sums (in all no more than the launch has: 896 threads of 72).
+    // strides) takes many instructions; roles are whole warpgroups then and share out the registers anew: to the
+    // epilogue's FP32 sums and 24 MMAs a slab, or to the loaders of 16-bit values, which keep two slabs (in all no more
+    // than the launch has: 896 threads of 72).
     static constexpr int kLoaders = TMA ? 2 : 16;
     static constexpr int kMmaWarp = kLoaders, kFixWarp = kLoaders + 1;
     static constexpr int kEpiWarp0 = !TMA ? kLoaders + 4 : RIGHT ? kLoaders + 2 : kLoaders + 1;
-    static constexpr int kLoaderRegs = 56, kMmaRegs = 72, kEpiRegs = 104;
-    static_assert(512 * kLoaderRegs + 128 * kMmaRegs + 256 * kEpiRegs <= 896 * 72, "register shares");
+    static constexpr int kLaunchRegs = 72;
+    static constexpr int kLoaderRegs = PLANES == 1 ? 88 : 56, kMmaRegs = PLANES == 1 ? 40 : 72, kEpiRegs = PLANES == 1 ? 56 : 104;
+    static_assert(512 * kLoaderRegs + 128 * kMmaRegs + 256 * kEpiRegs <= 896 * kLaunchRegs, "register shares");
     static constexpr int kEpiWarps = 8;
     static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
     static constexpr int kTmemCols = 2 * NT;
@@ -172,6 +174,26 @@ __device__ __forceinline__ void grouped_store16(const GroupedParams& p, long lon
     }
 }
 
+// This warpgroup's share of the registers from here on.
+template <int REGS, int LAUNCH>
+__device__ __forceinline__ void set_max_registers() {
+    if constexpr (REGS < LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+    if constexpr (REGS > LAUNCH) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// Loads of operands on their way through registers. Whole pieces of 16 bytes and more are not kept in L1, which is small
+// beside these tiles and holds what the roles spill; of odd rows, two loads share most lines.
+__device__ __forceinline__ uint32_t load_once(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_once(const uint16_t* p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+
 // Eight consecutive FP32 elements of a row in global memory.
 template <int ES>
 struct GroupedChunk {
@@ -186,19 +208,20 @@ struct GroupedChunk {
     __device__ __forceinline__ void load(const char* src, int align) {
         constexpr int kWords = 2 * ES;
         if (ES == 4 && align >= 32) {
-            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4 % kWords]), "=r"(w[5 % kWords]),
                            "=r"(w[6 % kWords]), "=r"(w[7 % kWords])
                          : "l"(src));
         } else if (align >= 16) {
 #pragma unroll
             for (int i = 0; i < kWords / 4; ++i) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+                asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                             : "l"(src + 16 * i));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+            for (int i = 0; i < kWords; ++i) w[i] = load_once(reinterpret_cast<const uint32_t*>(src) + i);
         }
     }
 
@@ -215,7 +238,7 @@ struct GroupedChunk {
         const int count = cols - col;
 #pragma unroll
         for (int i = 0; i < 7; ++i)
-            if (i < count) w[i % (2 * ES)] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+            if (i < count) w[i % (2 * ES)] = load_once(reinterpret_cast<const uint32_t*>(src) + i);
     }
 
     // Into 16 bytes of each plane at shared address `to`.
@@ -285,7 +308,7 @@ struct GroupedSide {
     }
 
     // The slab from d0 on of a contraction that ends at d1.
-    __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id) {
+    __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id, int /* slabs to the next load */) {
         if (o.inside() && d0 + kGroupedDepth <= d1) {
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
@@ -342,7 +365,7 @@ struct GroupedSide16 {
         at = o.base + row * o.ld + static_cast<long long>(col) * 2;
     }
 
-    __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id) {
+    __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id, int ahead) {
         const int lane = id % 32, warp = id / 32;
         const long long step = kApart * o.ld;
         // One element more than the segments have: a lane's word may end behind them.
@@ -350,11 +373,11 @@ struct GroupedSide16 {
             const uint32_t between = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at)) & 2u;
             shifted = between != 0;
             if (lane < kSegments && (MN || o.first + warp + lane * kApart < o.last))
-                edge = __ldg(reinterpret_cast<const uint16_t*>(at + lane * step));
+                edge = load_once(reinterpret_cast<const uint16_t*>(at + lane * step));
             const char* src = at + between + lane * 4;
 #pragma unroll
             for (int i = 0; i < kSegments; ++i, src += step)
-                if (MN || o.first + warp + i * kApart < o.last) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src));
+                if (MN || o.first + warp + i * kApart < o.last) w[i] = load_once(reinterpret_cast<const uint32_t*>(src));
         } else {
             shifted = false;
             const int col = (MN ? o.first + warp % kBoxes * 64 : d0) + 2 * lane, cols = MN ? o.last : d1;
@@ -364,11 +387,11 @@ struct GroupedSide16 {
 #pragma unroll
             for (int i = 0; i < kSegments; ++i, row += kApart, src += step / 2) {
                 w[i] = 0;
-                if (row < rows && col < cols) w[i] = __ldg(src);
-                if (row < rows && col + 1 < cols) w[i] |= static_cast<uint32_t>(__ldg(src + 1)) << 16;
+                if (row < rows && col < cols) w[i] = load_once(src);
+                if (row < rows && col + 1 < cols) w[i] |= load_once(src + 1) << 16;
             }
         }
-        at += MN ? kGroupedDepth * o.ld : kGroupedDepth * 2;
+        at += ahead * (MN ? kGroupedDepth * o.ld : kGroupedDepth * 2);
     }
 
     // Rows past the operand's end hold what they held: their results go nowhere.
@@ -568,14 +591,16 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (!Cfg::TMA && warp < Cfg::kLoaders) {
         // ------------------------------------------------------------ loader warps
-        // A slab's chunks of eight elements are dealt out to the threads; each keeps the next slab's in registers while
-        // it writes this one's. Where a slab lies inside the operand (all but edges) a chunk costs a pointer step and
+        // A slab's chunks are dealt out to the threads; each keeps the next slabs' in registers while it writes this
+        // one's. Where a slab lies inside the operand (all but edges) a chunk costs a pointer step and
         // its loads.
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kLoaderRegs));
+        set_max_registers<Cfg::kLoaderRegs, Cfg::kLaunchRegs>();
         using M = std::conditional_t<Cfg::ES == 2, GroupedSide16<Cfg, 128, Cfg::M_MN>, GroupedSide<Cfg, 128, Cfg::M_MN>>;
         using N = std::conditional_t<Cfg::ES == 2, GroupedSide16<Cfg, Cfg::NTC, Cfg::N_MN>, GroupedSide<Cfg, Cfg::NTC, Cfg::N_MN>>;
-        M m;
-        N n;
+        // Slabs ahead in registers: two of 16-bit values, since one does not cover a load's latency; FP32's are too wide.
+        constexpr int kAhead = PLANES == 1 ? 2 : 1;
+        M m[kAhead];
+        N n[kAhead];
         const int id = threadIdx.x;
         int it = 0;
         bool ok = true;
@@ -589,36 +614,43 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             auto n_place = [&] {
                 return typename N::Place{p.n_base, p.n_ld, p.n_align, t.r0 + half * rank, half, Cfg::RIGHT ? p.k : t.t1};
             };
-            m.start(m_place(), d0, id);
-            n.start(n_place(), d0, id);
-            if (t.kb > 0) {
-                m.load(m_place(), d0, d1, id);
-                n.load(n_place(), d0, d1, id);
-            }
-            for (int kb = 0; kb < t.kb; ++kb, ++it) {
+            auto load = [&](M& mk, N& nk, int kb) {
+                if (kb >= t.kb) return;
+                mk.load(m_place(), d0 + kb * kGroupedDepth, d1, id, kAhead);
+                nk.load(n_place(), d0 + kb * kGroupedDepth, d1, id, kAhead);
+            };
+            auto step_over = [&](M& mk, N& nk, int kb) {
                 const int s = it % STAGES;
                 ok = mbar_wait_bounded(&empty_bar[s], ((it / STAGES) & 1) ^ 1, limit, abort_flag);
                 ok = __all_sync(~0u, ok);
                 if (!ok) {
                     if (lane == 0) give_up(kStatusTimeoutProducer);
-                    break;
+                    return;
                 }
                 const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage);
-                m.store(m_tile, 128, id);
-                n.store(m_tile + Cfg::kMBytes, half, id);
+                mk.store(m_tile, 128, id);
+                nk.store(m_tile + Cfg::kMBytes, half, id);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full_bar[s]);
-                if (kb + 1 < t.kb) {
-                    m.load(m_place(), d0 + (kb + 1) * kGroupedDepth, d1, id);
-                    n.load(n_place(), d0 + (kb + 1) * kGroupedDepth, d1, id);
-                }
+                load(mk, nk, kb + kAhead);
+                ++it;
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                m[i].start(m_place(), d0 + i * kGroupedDepth, id);
+                n[i].start(n_place(), d0 + i * kGroupedDepth, id);
+                load(m[i], n[i], i);
+            }
+            for (int kb = 0; ok && kb < t.kb; kb += kAhead) {
+                step_over(m[0], n[0], kb);
+                if (kAhead == 2 && ok && kb + 1 < t.kb) step_over(m[kAhead - 1], n[kAhead - 1], kb + 1);
             }
         }
     } else if (!Cfg::TMA && warp > Cfg::kMmaWarp && warp < Cfg::kEpiWarp0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kMmaRegs));  // the rest of the MMA's warpgroup
+        set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();  // the rest of the MMA's warpgroup
     } else if (!Cfg::TMA && CG == 2 && warp == Cfg::kMmaWarp && !leader) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kMmaRegs));
+        set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();
         // ------------------------------------------------------------ tells the leader of the peer's filled stages
         if (lane == 0) {
             int it = 0;
@@ -637,7 +669,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (warp == Cfg::kMmaWarp) {
         // ------------------------------------------------------------ MMA issuer (leader)
-        if (!Cfg::TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kMmaRegs));
+        if (!Cfg::TMA) set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();
         if (lane == 0 && leader) {
             int it = 0, buf = 0;
             bool ok = true;
@@ -751,7 +783,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     } else if (warp >= Cfg::kEpiWarp0) {
         // ------------------------------------------------------------ epilogue
-        if (!Cfg::TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kEpiRegs));
+        if (!Cfg::TMA) set_max_registers<Cfg::kEpiRegs, Cfg::kLaunchRegs>();
         const int quarter = warp & 3;                    // TMEM lanes of this warp
         const int part = (warp - Cfg::kEpiWarp0) >> 2;   // which of every two 16-column chunks
         const uint32_t acc_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);

@@ -735,7 +735,7 @@ mfb_status_t gemv_int4_launch(const Int4Params& p, int device, cudaStream_t stre
     auto bulk = [&](const void* base, int size) {
         return aligned16(base) && (p.experts == 1 || static_cast<long long>(p.n) * p.groups * size % 16 == 0);
     };
-    bool s_bulk = bulk(p.scales, sizeof(TS)) && bulk(p.zeros, 1);
+    bool s_bulk = bulk(p.scales, sizeof(TS)) && (!p.zeros || bulk(p.zeros, 1));
     const long long tiles = static_cast<long long>(ids ? rows : 1) * ((p.n + 15) / 16);
     if (tiles > 0x7fffffffLL) return fail(MFB_EINVAL, "problem has too many output tiles");
     const unsigned grid = static_cast<unsigned>(std::min<long long>(tiles, sm_count(device)));

@@ -83,3 +83,38 @@ def test_train_store_decode(dtype):
     exact = (d1 - w1.detach().transpose(1, 2).float()).abs()
     # a clamped end of the range adds the rounding of the scale (its half step, 15 codes) and of the zero point
     assert (exact <= step * (1.0 + 15 * torch.finfo(dtype).eps / 2)).all()
+
+
+_FIRST_CALLS = """
+import torch, matrixflash_pro_b200 as mf
+x = torch.randn(40, 64, device="cuda").bfloat16()
+w = torch.randn(3, 64, 96, device="cuda").bfloat16()
+g = torch.randn(40, 96, device="cuda").bfloat16()
+off = torch.tensor([0, 10, 10, 40], dtype=torch.int32, device="cuda")
+ids = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = mf.grouped_matmul(x, w, off)
+    d = mf.grouped_matmul_backward_right(g, x, off)
+    q = mf.quantize_int4(w.transpose(1, 2).contiguous(), 32)
+    z = mf.gemv_int4(q, x[:2], experts=ids)
+    b = mf.dequantize_int4(q)
+graph.replay()
+mf.sync()
+ref = torch.cat([x[:10].double() @ w[0].double(), x[10:].double() @ w[2].double()])
+assert ((y.double() - ref).norm() / ref.norm()).item() < 4e-3
+ref = torch.stack([b[0].double() @ x[0].double(), b[2].double() @ x[1].double()])
+assert ((z.double() - ref).norm() / ref.norm()).item() < 8e-3
+print("captured")
+"""
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=root)
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALLS], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
