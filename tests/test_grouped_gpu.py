@@ -266,6 +266,26 @@ def test_positions_past_32_bits():
     _check(stack, *_reference_right(a, keep, off), 3)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_the_most_groups_and_many_rows(dtype):
+    """1024 groups, most of them empty, and more rows than a grid dimension holds."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    pick = torch.randint(0, 1024, (300,), generator=g, device="cuda") // 7 * 7
+    off = torch.searchsorted(pick.sort().values.contiguous(), torch.arange(1025, device="cuda")).int()
+    x, w = _normal((300, 48), dtype, 1), _normal((1024, 48, 40), dtype, 2)
+    _check(mf.grouped_matmul(x, w, off), *_reference(x, w, off), 48)
+    d = _normal((300, 40), dtype, 3)
+    _check(mf.grouped_matmul_backward_right(d, x, off), *_reference_right(x, d, off), 300)
+    x, w = _normal((70001, 16), dtype, 4), _normal((2, 16, 24), dtype, 5)
+    off = _offsets([65537, 4464])
+    _check(mf.grouped_matmul(x, w, off), *_reference(x, w, off), 16)
+    d = _normal((70001, 24), dtype, 6)
+    y, s = _reference_right(x, d, off)
+    got = mf.grouped_matmul_backward_right(d, x, off)
+    _check(got, y, s, 70001)
+
+
 @pytest.mark.parametrize("bad", [[0, 5, 3, 10], [-4, 2, 2, 6], [0, 4, 4, 99], [20, 20, 20, 20], [9, 0, 0, 0]])
 def test_bad_offsets_are_clamped_and_reported(bad):
     x, g, w = _normal((10, 16), F32, 1), _normal((10, 24), F32, 2), _normal((3, 16, 24), F32, 3)
