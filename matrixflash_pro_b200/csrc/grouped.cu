@@ -188,8 +188,11 @@ mfb_status_t launch_grouped(int device, const mfb_grouped_desc& d, cudaStream_t 
 
     const bool m_mn = !d.trans_b;
     const bool tma = size == 2 && p.m_align >= 16 && p.n_align >= 16 && d.groups > 0 && d.k > 0 && d.rows > 0;
-    // Rows of C per matrix: few of them leave a wide tile mostly empty, and the weights are what costs.
-    const bool wide = (right ? d.k : d.rows / std::max(1, d.groups)) > 64;
+    // Wide tiles take up to 256 rows of C (FP32: 128) per SM pair, narrow ones 64 per SM. 8 experts of 2048x4096, us,
+    // narrow / wide, by rows per group: 16 27.0 / 28.2, 48 28.3 / 29.9, 64 37.7 / 30.3, 128 55.7 / 32.3 (bf16);
+    // 16 127 / 128, 48 128 / 130, 64 177 / 131 (FP32): a group of more than 64 rows reads its weights twice in narrow
+    // tiles. Gradient by the matrices, 8 groups of 256 rows, n = 2048, by k: 64 7.0 / 9.0, 128 8.8 / 9.0, 256 12.7 / 9.8.
+    const bool wide = right ? d.k > 64 : d.rows / std::max(1, d.groups) > 48;
     const GroupedEntry e = size == 2 ? (tma ? entry_of<1, true>(right, m_mn, wide) : entry_of<1, false>(right, m_mn, wide))
                            : d.precision == MFB_PRECISION_FP32 ? entry_of<3, false>(right, m_mn, wide)
                                                                : entry_of<2, false>(right, m_mn, wide);

@@ -277,7 +277,7 @@ struct GroupedSide {
     static constexpr int kPerRow = MN ? WIDTH / 8 : 8;
     static constexpr int kChunks = (WIDTH * 8 + kThreads - 1) / kThreads;
     static constexpr int kApart = kThreads / kPerRow;  // rows between a thread's chunks
-    static constexpr int kPlane = WIDTH * 128;
+    static constexpr int kPlane = WIDTH * 128, kPrefetch = 4;
     GroupedChunk<ES> c[kChunks];
     const char* at[MN ? 1 : kChunks];  // this thread's chunks of the next slab
 
@@ -310,6 +310,16 @@ struct GroupedSide {
     // The slab from d0 on of a contraction that ends at d1.
     __device__ __forceinline__ void load(const Place& o, int d0, int d1, int id, int /* slabs to the next load */) {
         if (o.inside() && d0 + kGroupedDepth <= d1) {
+            // The lines of a later slab on their way into L2: one slab in registers covers its latency, not HBM's.
+            if (id % 4 == 0 && d0 + (kPrefetch + 1) * kGroupedDepth <= d1) {
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) {
+                    if (!has(i, id) || (!MN && i * kApart >= o.width)) continue;
+                    const char* later = MN ? at[0] + (i * kApart + kPrefetch * kGroupedDepth) * o.ld
+                                           : at[MN ? 0 : i] + kPrefetch * kGroupedDepth * ES;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(later));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 if (!has(i, id)) continue;
