@@ -48,17 +48,21 @@ mfb_status_t validate_grouped(const mfb_grouped_desc* d, const int* offsets, con
     if (right && d->groups > 1 && d->stride < (c_rows - 1) * d->ldc + d->n)
         return fail(MFB_EINVAL, "stride makes the groups' outputs overlap");
     if (!c) return fail(MFB_EINVAL, "null C pointer");
-    // Extents in bytes: the output may not overlap an operand.
     const long long b_rows = right ? d->rows : d->trans_b ? d->n : d->k;
+    // Extents in bytes: the output may not overlap what the kernel reads.
+    const char* cs = static_cast<const char*>(c);
+    const char* c_end = cs + extent(c_rows, d->ldc, d->n, right ? d->groups : 1, right ? d->stride : 0,
+                                    dtype_bytes(d->out_dtype));
+    const char* os = reinterpret_cast<const char*>(offsets);
+    if (cs < os + 4 * (d->groups + 1ll) && os < c_end)
+        return fail(MFB_EINVAL, "the output of a grouped product cannot alias the offsets");
+    if (reinterpret_cast<uintptr_t>(offsets) % 4) return fail(MFB_EINVAL, "offsets must be aligned to 4 bytes");
     const bool reads = d->rows > 0 && d->k > 0 && d->groups > 0;
     if (!reads) return MFB_OK;
     if (!a || !b) return fail(MFB_EINVAL, "null A or B pointer");
-    const char* cs = static_cast<const char*>(c);
     const char* as = static_cast<const char*>(a);
     const char* bs = static_cast<const char*>(b);
     const int size = dtype_bytes(d->dtype);
-    const char* c_end = cs + extent(c_rows, d->ldc, d->n, right ? d->groups : 1, right ? d->stride : 0,
-                                    dtype_bytes(d->out_dtype));
     const char* a_end = as + extent(d->rows, d->lda, d->k, 1, 0, size);
     const char* b_end = bs + extent(b_rows, d->ldb, b_cols, right ? 1 : d->groups, right ? 0 : d->stride, size);
     if ((cs < a_end && as < c_end) || (cs < b_end && bs < c_end))

@@ -836,6 +836,23 @@ mfb_status_t validate_rows(const Int4Params& p, const void* w, int dtype, long l
     return MFB_OK;
 }
 
+bool overlap(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
+
+// Whether [at, at + bytes) reaches into the codes, scales or zero points.
+bool overlaps_matrix(const Int4Params& p, int scale_dtype, const void* at, long long bytes) {
+    const long long scales = p.rows * p.groups;
+    return overlap(at, bytes, p.packed, p.rows * p.row_bytes) ||
+           overlap(at, bytes, p.scales, scales * dtype_bytes(scale_dtype)) || overlap(at, bytes, p.zeros, scales);
+}
+
+// Bytes from the first to behind the last element of `m`'s rows in a caller's matrix.
+long long rows_extent(const Int4Params& p, int dtype, long long ld, long long stride) {
+    return ((p.n - 1ll) * ld + (p.experts - 1ll) * stride + p.k) * dtype_bytes(dtype);
+}
+
 }  // namespace
 }  // namespace mfb
 
@@ -851,6 +868,8 @@ MFB_API mfb_status_t mfb_quantize_int4(int device, mfb_stream_t stream, const vo
     MFB_TRY(validate_dtype(dtype));
     if (p.rows == 0 || p.k == 0) return MFB_OK;
     MFB_TRY(validate_rows(p, w, dtype, ldw, stride_w, false));
+    if (overlaps_matrix(p, out->scale_dtype, w, rows_extent(p, dtype, ldw, stride_w)))
+        return fail(MFB_EINVAL, "a 4-bit matrix cannot alias the weights that it is made from");
     DeviceGuard guard;
     MFB_TRY(select_device(device));
     const int cells = p.groups * (p.group / 16);  // whole groups, so that a group's lanes are in one warp
@@ -881,6 +900,8 @@ MFB_API mfb_status_t mfb_dequantize_int4(int device, mfb_stream_t stream, const 
     MFB_TRY(validate_dtype(dtype));
     if (p.rows == 0 || p.k == 0) return MFB_OK;
     MFB_TRY(validate_rows(p, out, dtype, ldo, stride_o, true));
+    if (overlaps_matrix(p, m->scale_dtype, out, rows_extent(p, dtype, ldo, stride_o)))
+        return fail(MFB_EINVAL, "the weights of a 4-bit matrix cannot alias its parts");
     DeviceGuard guard;
     MFB_TRY(select_device(device));
     const int cells = p.row_bytes / 8;
@@ -913,11 +934,12 @@ MFB_API mfb_status_t mfb_gemv_int4(int device, mfb_stream_t stream, const mfb_in
     if (reinterpret_cast<uintptr_t>(x) % dtype_bytes(dtype) || reinterpret_cast<uintptr_t>(y) % dtype_bytes(dtype))
         return fail(MFB_EINVAL, "x and y must be aligned to their type");
     if (ldx < 0 || (rows > 1 && ldy < p.n)) return fail(MFB_EINVAL, "the row stride of y is smaller than n");
-    const char* xs = static_cast<const char*>(x);
-    const char* ys = static_cast<const char*>(y);
-    if (p.k > 0 && ys < xs + ((rows - 1) * ldx + p.k) * dtype_bytes(dtype) &&
-        xs < ys + ((rows - 1) * ldy + p.n) * dtype_bytes(dtype))
+    if (reinterpret_cast<uintptr_t>(expert_ids) % 4) return fail(MFB_EINVAL, "expert ids must be aligned to 4 bytes");
+    const long long y_bytes = ((rows - 1) * ldy + p.n) * dtype_bytes(dtype);
+    if (p.k > 0 && overlap(y, y_bytes, x, ((rows - 1) * ldx + p.k) * dtype_bytes(dtype)))
         return fail(MFB_EINVAL, "GEMV output cannot alias x");
+    if (overlaps_matrix(p, m->scale_dtype, y, y_bytes) || overlap(y, y_bytes, expert_ids, 4ll * rows))
+        return fail(MFB_EINVAL, "GEMV output cannot alias the matrix or the expert ids");
     DeviceGuard guard;
     MFB_TRY(select_device(device));
     return with_dtype(m->scale_dtype, [&](auto ts) {

@@ -88,3 +88,11 @@ def test_abi_rejects_pointers_and_aliases():
     # nothing to do needs no device
     assert lib.mfb_grouped_gemm(0, None, ctypes.byref(_desc(rows=0)), O, 0, 0, 0) == _lib.MFB_OK
     assert right(0, None, ctypes.byref(_desc(groups=0)), O, 0, 0, 0) == _lib.MFB_OK
+
+
+def test_abi_rejects_outputs_over_the_offsets():
+    lib = mf.lib()
+    for entry in (lib.mfb_grouped_gemm, lib.mfb_grouped_gemm_bwd_right):
+        for offsets, needle in ((C, "alias"), (C + 4, "alias"), (C - 4, "alias"), (C - 4096 + 2, "aligned")):
+            assert entry(0, None, ctypes.byref(_desc()), offsets, A, B, C) == _lib.MFB_EINVAL
+            assert needle in _lib.last_error()

@@ -90,3 +90,17 @@ def test_abi_rejects_operands():
     refused(lib.mfb_quantize_int4(0, None, X + 1, 1, 64, 0, m), "aligned")
     assert lib.mfb_gemv_int4(0, None, m, 0, 0, 0, 0, 0, 0, 0) == _lib.MFB_OK
     assert lib.mfb_dequantize_int4(0, None, ctypes.byref(_matrix(n=0)), 0, 0, 0, 0) == _lib.MFB_OK
+
+
+@pytest.mark.parametrize("at", [P, P + 4 * 32 - 4, S, S + 4 * 2 * 4 - 4, Z, Z + 4, P - 12])
+def test_abi_rejects_outputs_over_the_matrix(at):
+    # 4 rows of 64 codes, 2 scales and 2 zero points; y takes 16 bytes, the weights 1024
+    lib = mf.lib()
+    m = ctypes.byref(_matrix())
+    for st in (lib.mfb_gemv_int4(0, None, m, 1, X, 64, 0, 0, at, 4), lib.mfb_dequantize_int4(0, None, m, at, 0, 64, 0),
+               lib.mfb_quantize_int4(0, None, at, 0, 64, 0, m)):
+        assert st == _lib.MFB_EINVAL and "alias" in _lib.last_error()
+    assert lib.mfb_gemv_int4(0, None, m, 1, X, 64, 0, Y + 12, Y, 4) == _lib.MFB_EINVAL
+    assert "alias" in _lib.last_error()
+    assert lib.mfb_gemv_int4(0, None, m, 1, X, 64, 0, Y + 66, Y, 4) == _lib.MFB_EINVAL
+    assert "aligned" in _lib.last_error()
