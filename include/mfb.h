@@ -325,7 +325,8 @@ typedef enum mfb_dtype_t { MFB_DTYPE_F32 = 0, MFB_DTYPE_F16 = 1, MFB_DTYPE_BF16 
  * [offsets[e], offsets[e + 1]), which may be none. They are read by the kernels, so the host
  * needs no group size and a captured graph follows new offsets on replay. Offsets below 0,
  * above `rows` or smaller than an earlier one are clamped (nothing out of bounds is touched)
- * and reported as MFB_EINVAL by the next mfb_sync / mfb_device_status. groups <= 1024. */
+ * and reported as MFB_EINVAL by the next mfb_sync / mfb_device_status. groups <= 1024.
+ * C may overlap neither A, B nor the offsets. */
 typedef struct mfb_grouped_desc {
     int groups; /* experts */
     int rows;   /* rows of A (and of C, or of B in mfb_grouped_gemm_bwd_right) */
@@ -356,7 +357,8 @@ MFB_API mfb_status_t mfb_grouped_gemm_bwd_right(int device, mfb_stream_t stream,
 /* n x k weights (or a stack of `experts` of them) as 4-bit codes q with one scale s (and zero point
  * z, 8 where `zeros` is NULL) per row and group of `group` consecutive columns: w = (q - z) * s.
  * Column j of a row is in byte j / 2, even j in the low half; rows take 16 * ceil(k / 32) bytes
- * (what is behind column k is ignored); scales and zeros are n x ceil(k / group), all contiguous. */
+ * (what is behind column k is ignored); scales and zeros are n x ceil(k / group), all contiguous.
+ * No output may overlap what the same call reads. */
 typedef struct mfb_int4_matrix {
     unsigned char* packed;  /* 16-byte aligned */
     void* scales;           /* scale_dtype */

@@ -13,7 +13,8 @@ With transpose_right the weights (and their gradient) are stored [e,n,k].
 Operands are float32 (strict, as GemmPrecision.fp32; tf32 permits fewer terms), float16 or
 bfloat16 CUDA tensors of one type with unit stride in the last dimension; rows and matrices may be
 padded or shared (strides are taken from the tensors, 0 between matrices reuses one weight). Sums
-are FP32, rounded once; an infinite float32 operand gives NaN (it has no terms to split into). `out` may be given, of the operands' type or float32.
+are FP32, rounded once; an infinite float32 operand gives NaN (it has no terms to split into).
+`out` may be given, of the operands' type or float32, and may overlap nothing that the call reads.
 
 offsets is a contiguous int32 CUDA tensor of e + 1 entries that the kernels read: the host never
 waits for group sizes, and a captured graph follows new offsets on replay. Rows in front of

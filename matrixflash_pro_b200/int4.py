@@ -14,7 +14,8 @@ column j of a row in byte j // 2, even j in the low four bits, whatever is behin
 ignored; `scales` (float32, float16 or bfloat16) and `zeros` (uint8, 0..15) are contiguous
 [.., n, ceil(k / group)].
 
-The work goes to `stream`, by default the current stream of the matrix's device.
+A given `out` may overlap nothing that the call reads. The work goes to `stream`, by default the
+current stream of the matrix's device.
 """
 from __future__ import annotations
 
