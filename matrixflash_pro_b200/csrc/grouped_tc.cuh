@@ -17,9 +17,13 @@
 // three). Products hh, hm, mh, mm, hl, lh are kept (six MMAs per step, 1/6 of the BF16 rate); what is left
 // out is below 2^-21 of |a b|. Two terms (TF32 precision) keep hh, hm, mh.
 //
-// The tensor core adds with truncation, so strict FP32 restarts the accumulator every 64 of the
-// contraction and the epilogue warps add the chunks in registers, rounding to nearest (every 128 instead
-// would save 5% of the time and take the error at k = 4096 from 1.9e-7 to 6e-7).
+// The tensor core adds with truncation, so the accumulator restarts every 64 of the contraction (strict FP32) or 512
+// (all others) and the epilogue warps add the chunks, rounding to nearest: the error does not grow with the
+// contraction. (FP32 every 128 instead would save 5% of the time and take the error at k = 4096 from 1.9e-7 to 6e-7.)
+// 16-bit operands, k = 4096, 8 experts of 1024 rows, by the chunk: 256 662 us, error of the sums 2.4e-7 (all products
+// positive 3.8e-7); 512 589 us, 4.8e-7 (9e-7); 1024 573 us, 1e-6 (2.2e-6); never restarted 552 us, 4.4e-6 (1.4e-5,
+// and 8e-5 at k = 16384). 512 is the longest that stays below 1e-6. What it costs is the hand-over: the next chunk's MMAs
+// wait for a buffer whose reader needs 3600 cycles, signals across the pair included, and a chunk's MMAs take 4096.
 //
 // Bounds, and what it reaches on a B200: 8192 rows over 8 experts, 4096x11008 bf16, 539 us, 1370 TFLOP/s, the
 // tensor core under the power limit (cuBLAS sustains 1387); 32 rows over 32 experts, 2048x1024 bf16, 25.8 us,
@@ -73,6 +77,7 @@ struct GroupedConfig {
     static constexpr int kMBytes = PLANES * kMPlane, kNBytes = PLANES * kNPlane;
     static constexpr int kSlab = kMBytes + kNBytes;
     static constexpr int kStage = KS * kSlab;
+    static constexpr int kSumStages = PLANES == 3 ? 1 : 512 / (kGroupedDepth * KS);  // stages per accumulator chunk
     static constexpr int kBarriers = STAGES * kStage;
     static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 6) + 8;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
@@ -88,7 +93,10 @@ struct GroupedConfig {
     static_assert(512 * kLoaderRegs + 128 * kMmaRegs + 256 * kEpiRegs <= 896 * kLaunchRegs, "register shares");
     static constexpr int kEpiWarps = 8;
     static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-    static constexpr int kTmemCols = 2 * NT;
+    // The chunks' sums stay in registers, or, where the loaders need those, in TMEM beside as many accumulators as fit.
+    static constexpr bool kTmemSums = !TMA && PLANES == 1;
+    static constexpr int kBuffers = kTmemSums && NT == 256 ? 1 : 2;  // accumulators
+    static constexpr int kTmemCols = (kBuffers + (kTmemSums ? 1 : 0)) * NT <= 2 * NT ? 2 * NT : 4 * NT;
     // N of an MMA is a multiple of this: whole 64-column boxes per CTA where the N side is MN-major.
     static constexpr int kGranule = (RIGHT ? 64 : 16) * CG;
     // Arrivals that complete a filled stage, besides the bytes of TMA copies: the loader warps', and in the leader of
@@ -677,9 +685,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     umma_idesc_f16(Cfg::BM, t.cols, Cfg::M_MN, Cfg::N_MN, PLANES > 1 ? 1 : p.bf16);
                 uint32_t d_tmem = 0, acc = 0;
                 for (int kb = 0; kb < t.kb; ++kb, ++it) {
-                    if (PLANES == 3 || kb == 0) {
-                        const int b = buf & 1;
-                        if (!mbar_wait_bounded(&acc_empty_bar[b], ((buf >> 1) & 1) ^ 1, limit, abort_flag)) {
+                    if (kb % Cfg::kSumStages == 0) {
+                        const int b = buf % Cfg::kBuffers;
+                        if (!mbar_wait_bounded(&acc_empty_bar[b], (buf / Cfg::kBuffers & 1) ^ 1, limit, abort_flag)) {
                             give_up(kStatusTimeoutMma);
                             ok = false;
                             break;
@@ -727,9 +735,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     }
                     if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
                     else umma_commit(&empty_bar[s]);
-                    if (PLANES == 3 || kb == t.kb - 1) {
-                        if (CG == 2) umma_commit_pair(&acc_full_bar[buf & 1], 0x3);
-                        else umma_commit(&acc_full_bar[buf & 1]);
+                    if (kb % Cfg::kSumStages == Cfg::kSumStages - 1 || kb == t.kb - 1) {
+                        if (CG == 2) umma_commit_pair(&acc_full_bar[buf % Cfg::kBuffers], 0x3);
+                        else umma_commit(&acc_full_bar[buf % Cfg::kBuffers]);
                         ++buf;
                     }
                 }
@@ -784,7 +792,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         // ------------------------------------------------------------ epilogue
         if (!Cfg::TMA) set_max_registers<Cfg::kEpiRegs, Cfg::kLaunchRegs>();
         const int quarter = warp & 3;                    // TMEM lanes of this warp
-        const int part = (warp - Cfg::kEpiWarp0) >> 2;   // which of every two 16-column chunks
+        const int part = (warp - Cfg::kEpiWarp0) >> 2;   // which of every two 16-column pieces
         const uint32_t acc_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         int buf = 0;
         bool ok = true;
@@ -802,21 +810,39 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 for (int q = part; q * 16 < t.cols; q += 2) store(q, zero);
                 continue;
             }
-            constexpr int kChunks = NT / 32;
-            if constexpr (PLANES == 3) {
-                float sum[kChunks][16];
+            constexpr int kPieces = NT / 32;
+            float sum[Cfg::kTmemSums ? 1 : kPieces][16];
+            if constexpr (!Cfg::kTmemSums) {
 #pragma unroll
-                for (int i = 0; i < kChunks; ++i)
+                for (int i = 0; i < kPieces; ++i)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) sum[i][j] = 0.0f;
-                for (int kb = 0; kb < t.kb; ++kb, ++buf) {
-                    const int b = buf & 1;
-                    ok = mbar_wait_bounded(&acc_full_bar[b], (buf >> 1) & 1, limit, abort_flag);
-                    ok = __all_sync(~0u, ok);
-                    if (!ok) break;
-                    tc_fence_after();
+            }
+            const uint32_t sums = acc_base + Cfg::kBuffers * NT;
+            for (int kb = 0; kb < t.kb; kb += Cfg::kSumStages, ++buf) {
+                const int b = buf % Cfg::kBuffers;
+                ok = mbar_wait_bounded(&acc_full_bar[b], buf / Cfg::kBuffers & 1, limit, abort_flag);
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                tc_fence_after();
+                if constexpr (Cfg::kTmemSums) {
+                    for (int q = part; q * 16 < t.cols; q += 2) {
+                        uint32_t v[16], o[16];
+                        tmem_ld_32x32b_x16(acc_base + b * NT + q * 16, v);
+                        if (kb) tmem_ld_32x32b_x16(sums + q * 16, o);
+                        tmem_ld_wait();
+                        tmem_regs_ready(v);
+                        if (kb) {
+                            tmem_regs_ready(o);
 #pragma unroll
-                    for (int i = 0; i < kChunks; ++i) {
+                            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(v[j]));
+                        }
+                        tmem_st_32x32b_x16(sums + q * 16, v);
+                    }
+                    tmem_st_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
                         const int q = 2 * i + part;
                         if (q * 16 < t.cols) {
                             uint32_t v[16];
@@ -827,35 +853,26 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             for (int j = 0; j < 16; ++j) sum[i][j] += __uint_as_float(v[j]);
                         }
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_leader(&acc_empty_bar[b]);
                 }
-                if (ok) {
-#pragma unroll
-                    for (int i = 0; i < kChunks; ++i)
-                        if ((2 * i + part) * 16 < t.cols) store(2 * i + part, sum[i]);
-                }
-            } else {
-                const int b = buf & 1;
-                ok = mbar_wait_bounded(&acc_full_bar[b], (buf >> 1) & 1, limit, abort_flag);
-                ok = __all_sync(~0u, ok);
-                if (ok) {
-                    tc_fence_after();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&acc_empty_bar[b]);
+            }
+            if (ok) {
+                if constexpr (Cfg::kTmemSums) {
                     for (int q = part; q * 16 < t.cols; q += 2) {
                         uint32_t v[16];
-                        tmem_ld_32x32b_x16(acc_base + b * NT + q * 16, v);
+                        tmem_ld_32x32b_x16(sums + q * 16, v);
                         tmem_ld_wait();
                         tmem_regs_ready(v);
-                        float x[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]);
-                        store(q, x);
+                        for (int j = 0; j < 16; ++j) sum[0][j] = __uint_as_float(v[j]);
+                        store(q, sum[0]);
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_leader(&acc_empty_bar[b]);
-                    ++buf;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i)
+                        if ((2 * i + part) * 16 < t.cols) store(2 * i + part, sum[i]);
                 }
             }
             if (!ok && lane == 0) give_up(kStatusTimeoutEpilogue);

@@ -386,3 +386,29 @@ def test_refusals_on_device_tensors():
         mf.grouped_matmul_backward_right(x, x, off, out=torch.empty(1, 8, 8, device="cuda").expand(2, 8, 8))
     with pytest.raises(ValueError):
         mf.grouped_matmul(x, w, off, precision=5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("cut", [0, 1])
+@pytest.mark.parametrize("sizes", [[70, 130, 3], [20, 9]], ids=str)
+def test_long_sums_of_16_bit_operands_do_not_drift(dtype, cut, sizes):
+    """All products positive and FP32 outputs. Within 512 of the contraction the tensor core truncates, twice per 16:
+    2 * 32 U of that chunk's sum; chunks are added with rounding, U / 2 of the sum each: U (64 + k / 1024) S in all, 80 U S
+    = 9.5e-6 S at k = 16384. Truncation over the whole contraction takes 8e-5."""
+    k, n, rows = 16384, 136, sum(sizes)
+    off = _offsets(sizes)
+    bound = lambda s: U * (64 + k / 1024) * s  # noqa: E731
+    x = _normal((rows, k + 8), dtype, 1).abs()[:, cut:cut + k]
+    w = _normal((len(sizes), n, k + 8), dtype, 2).abs()[:, :, cut:cut + k]
+    out = torch.empty(rows, n, device="cuda")
+    y, s = _reference(x, w.transpose(1, 2), off)
+    assert ((mf.grouped_matmul(x, w, off, True, out=out).double() - y).abs() <= bound(s)).all()
+    v = _normal((len(sizes), k, n + 8), dtype, 3).abs()[:, :, cut:cut + n]
+    y, s = _reference(x, v, off)
+    assert ((mf.grouped_matmul(x, v, off, out=out).double() - y).abs() <= bound(s)).all()
+    a, g = _normal((k, sizes[0] + 8), dtype, 4).abs()[:, cut:cut + sizes[0]], _normal((k, 80), dtype, 5).abs()[:, cut:cut + 72]
+    off = _offsets([k])
+    dw = torch.empty(1, sizes[0], 72, device="cuda")
+    y, s = _reference_right(a, g, off)
+    assert ((mf.grouped_matmul_backward_right(g, a, off, out=dw).double() - y).abs() <= bound(s)).all()
+    mf.sync()
