@@ -79,7 +79,7 @@ struct GroupedConfig {
     static constexpr int kStage = KS * kSlab;
     static constexpr int kSumStages = PLANES == 3 ? 1 : 512 / (kGroupedDepth * KS);  // stages per accumulator chunk
     static constexpr int kBarriers = STAGES * kStage;
-    static constexpr int kTables = kBarriers + 8 * (3 * STAGES + 6) + 8;
+    static constexpr int kTables = kBarriers + 8 * (4 * STAGES + 5) + 8;
     static constexpr int kSmem = kTables + 8 * (kGroupedMaxGroups + 1) + 1024;
     // Warps. TMA: one producer per operand. Else 16 loader warps, since turning FP32 into three terms (or reading odd
     // strides) takes many instructions; roles are whole warpgroups then and share out the registers anew: to the
@@ -429,11 +429,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kBarriers);  // of the leader: both CTAs' stage is filled
     uint64_t* empty_bar = full_bar + STAGES;
     uint64_t* tail_bar = empty_bar + STAGES;  // a stage whose last rows are still to be cleared
-    uint64_t* acc_full_bar = tail_bar + STAGES;
+    // In the leader: the peer's tail in this stage is cleared. One per stage, like tail_bar, so that no arrival is lost:
+    // the peer's next tail there is loaded only after the MMA has consumed the stage, which it does after the leader
+    // has waited for this one. (With one barrier for all stages the peer could clear two tails in different stages
+    // before the leader waits for the first, whose phase would be over unseen.)
+    uint64_t* peer_tail_bar = tail_bar + STAGES;
+    uint64_t* acc_full_bar = peer_tail_bar + STAGES;
     uint64_t* acc_empty_bar = acc_full_bar + 2;  // used in the leader
     uint64_t* drain_bar = acc_empty_bar + 2;
-    uint64_t* peer_tail_bar = drain_bar + 1;  // in the leader: the peer's tail is cleared
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(peer_tail_bar + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* offset = reinterpret_cast<int*>(smem + Cfg::kTables);
     int* first_tile = offset + kGroupedMaxGroups + 1;
@@ -449,13 +453,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             mbar_init(&full_bar[s], Cfg::full_count(leader));
             mbar_init(&empty_bar[s], 1);
             mbar_init(&tail_bar[s], 1);
+            mbar_init(&peer_tail_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full_bar[b], 1);
             mbar_init(&acc_empty_bar[b], CG * Cfg::kEpiWarps);
         }
         mbar_init(drain_bar, 1);
-        mbar_init(peer_tail_bar, 1);
         *abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async_smem();
@@ -751,14 +755,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         // The last MMA step of a contraction over a group's rows may hold rows of the next group (or NaN of a
         // buffer's spare rows): both operands' become 0 before the MMA may read them.
         int it = 0;
-        uint32_t phases = 0, peer_phase = 0;  // parities of each stage's tail barrier, of the peer's
+        uint32_t phases = 0;  // parities of each stage's tail barriers
         bool ok = true;
         while (ok && work.next(t)) {
             const int rows = t.t1 - t.t0, valid = rows % kGroupedDepth, end = (valid + 15) / 16 * 16;
             it += t.kb;
             if (rows % 16 == 0) continue;
             const int s = (it - 1) % STAGES;
-            ok = mbar_wait_bounded(&tail_bar[s], (phases >> s) & 1, limit, abort_flag);
+            const uint32_t phase = (phases >> s) & 1;
+            ok = mbar_wait_bounded(&tail_bar[s], phase, limit, abort_flag);
             ok = __all_sync(~0u, ok);
             if (!ok) {
                 if (lane == 0) give_up(kStatusTimeoutProducer);
@@ -775,12 +780,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             __syncwarp();
             // One arrival completes the stage: the leader's, after the peer's tail is cleared too.
             if (CG == 2 && !leader) {
-                if (lane == 0) mbar_arrive_cluster(leader_bar(peer_tail_bar));
+                if (lane == 0) mbar_arrive_cluster(leader_bar(&peer_tail_bar[s]));
                 continue;
             }
             if (CG == 2) {
-                ok = __all_sync(~0u, mbar_wait_bounded(peer_tail_bar, peer_phase, limit, abort_flag));
-                peer_phase ^= 1;
+                ok = __all_sync(~0u, mbar_wait_bounded(&peer_tail_bar[s], phase, limit, abort_flag));
                 if (!ok) {
                     if (lane == 0) give_up(kStatusTimeoutProducer);
                     break;

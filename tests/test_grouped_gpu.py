@@ -412,3 +412,22 @@ def test_long_sums_of_16_bit_operands_do_not_drift(dtype, cut, sizes):
     y, s = _reference_right(a, g, off)
     assert ((mf.grouped_matmul_backward_right(g, a, off, out=dw).double() - y).abs() <= bound(s)).all()
     mf.sync()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("groups,most,k,n", [(64, 40, 512, 1000), (512, 40, 72, 128), (256, 250, 128, 640), (64, 250, 512, 640)])
+def test_weight_gradient_of_many_ragged_groups(dtype, groups, most, k, n):
+    """Six and more tiles per SM pair, nearly all of them ending inside a 16-row step and one or two stages long, so that
+    cleared rows of consecutive tiles are handed over in quick succession; for n = 128 and 640 the second SM's half of
+    some tiles lies outside the operand and is filled sooner than the first's."""
+    g = torch.Generator()
+    g.manual_seed(groups + most)
+    off = _offsets(torch.randint(0, most // 2, (groups,), generator=g).mul(2).add(1).tolist())
+    rows = int(off[-1])
+    x, d = _normal((rows, k), dtype, 1), _normal((rows, n), dtype, 2)
+    mf.device_status()
+    first = mf.grouped_matmul_backward_right(d, x, off)
+    _check(first, *_reference_right(x, d, off), most)
+    for _ in range(10):
+        assert torch.equal(mf.grouped_matmul_backward_right(d, x, off), first)
+    assert mf.device_status() == 0
