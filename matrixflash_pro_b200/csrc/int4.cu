@@ -1,5 +1,6 @@
 // 4-bit weights: w = (q - z) * s with a scale s and zero point z per row and group of 32, 64 or 128
 // columns. Quantising, reading back, and the product with a few rows (decoding).
+#include "copy_ring.h"
 #include "mfb_internal.h"
 
 #include <cuda_bf16.h>
@@ -473,8 +474,7 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
     TS* scales = reinterpret_cast<TS*>(sums + (most << kw_log) * RT * 32);                     // [tile][16 rows][group]
     unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + most * 16 * p.groups);
     const bool whole = p.groups % kGroups == 0;  // every chunk has all its groups, vectors are aligned
-    int load_stage = 0, stage = 0;
-    uint32_t parity = 0;  // of the barriers' round that `stage` is in
+    CopyRing<kDepth> copies;
     uint32_t scale_parity = 0;
     bool ok = true;
     // An even share of all tiles: segment d, tiles m0 .. of it, left of them in all.
@@ -505,12 +505,13 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
             auto load = [&]() {
                 if (load_chunk >= chunks) return;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&bars[warp][load_stage], 1024 * HALVES);
-                    tma_load_2d(my_ring + load_stage * 64 * HALVES, &codes, &bars[warp][load_stage], load_chunk * 64 * HALVES,
+                    const unsigned s = copies.next();
+                    mbar_arrive_expect_tx(&bars[warp][s], 1024 * HALVES);
+                    tma_load_2d(my_ring + s * 64 * HALVES, &codes, &bars[warp][s], load_chunk * 64 * HALVES,
                                 box_row + load_tile * tw_count * 16);
                 }
+                ++copies.issued;
                 if (++load_tile == mine) load_tile = 0, load_chunk += kw_count;
-                if (++load_stage == kDepth) load_stage = 0;
             };
 #pragma unroll 1
             for (int i = 0; i < kDepth; ++i) load();
@@ -552,16 +553,18 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
             };
 
             uint32_t xb[HALVES][RT][4][kTerms][4];
-            // N tiles from tile j on: independent chains of MMAs side by side.
+            // N tiles from tile j on: independent chains of MMAs side by side. A wait that gives up ends it for the whole
+            // warp, before anything is read or another copy started.
             auto step_over = [&](auto n_, int j, int chunk) {
                 constexpr int N = decltype(n_)::value;
                 const uint32_t* box[N];
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
-                    ok = ok && mbar_wait_bounded(&bars[warp][stage], parity, wait_limit_ns, nullptr);
-                    box[u] = reinterpret_cast<const uint32_t*>(my_ring + stage * 64 * HALVES);
-                    if (++stage == kDepth) stage = 0, parity ^= 1;
+                    ok = ok && mbar_wait_bounded(&bars[warp][copies.stage(u)], copies.parity(u), wait_limit_ns, nullptr);
+                    box[u] = reinterpret_cast<const uint32_t*>(my_ring + copies.stage(u) * 64 * HALVES);
                 }
+                ok = __all_sync(~0u, ok);
+                if (!ok) return;
                 float acc[N][RT][4];
 #pragma unroll
                 for (int b = 0; b < HALVES; ++b) {
@@ -591,6 +594,7 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
                         }
                     if (b == HALVES - 1) {
                         __syncwarp();  // every lane has read the boxes
+                        copies.consumed += N;
 #pragma unroll
                         for (int u = 0; u < N; ++u) load();
                     }
@@ -671,12 +675,8 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
                     scales_here = true;
                 }
                 int j = 0;
-                for (; ok && j + 2 <= mine; j += 2) {
-                    step_over(std::integral_constant<int, 2>(), j, chunk);
-                    ok = __all_sync(~0u, ok);
-                }
+                for (; ok && j + 2 <= mine; j += 2) step_over(std::integral_constant<int, 2>(), j, chunk);
                 if (ok && j < mine) step_over(std::integral_constant<int, 1>(), j, chunk);
-                ok = __all_sync(~0u, ok);
             }
             if (!ok && lane == 0) report_status(kStatusTimeoutProducer, nullptr);
             ok = __syncthreads_and(ok);
@@ -698,11 +698,11 @@ __global__ void __launch_bounds__(32 * kGemvWarps, 1)
         scale_parity ^= 1;  // one copy of scales per round of tiles
     }
     // A wait that gave up leaves copies in flight; they land (or the limit passes) before the block ends.
-    while (!ok && stage != load_stage) {
-        if (!mbar_wait_drain(&bars[warp][stage], parity, wait_limit_ns)) break;
-        if (++stage == kDepth) stage = 0, parity ^= 1;
+    if (!ok) {
+        bool landed = copies.drain([&](unsigned s, unsigned parity) { return mbar_wait_drain(&bars[warp][s], parity, wait_limit_ns); });
+        if (left > 0 && s_bulk && threadIdx.x == 0) landed = mbar_wait_drain(&scale_bar, scale_parity, wait_limit_ns) && landed;
+        if (!landed) report_status(kStatusTimeoutDrain, nullptr);
     }
-    while (!ok && left > 0 && s_bulk && threadIdx.x == 0 && !mbar_wait_drain(&scale_bar, scale_parity, wait_limit_ns)) break;
     if (seg.begin[seg.count] < rows)  // rows of no expert
         for (int r = 0; r < rows; ++r) {
             const int e = ids[r];
