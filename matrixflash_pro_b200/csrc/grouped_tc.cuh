@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 for (int kb = 0; kb < t.kb; ++kb, ++it) {
                     if (kb % Cfg::kSumStages == 0) {
                         const int b = buf % Cfg::kBuffers;
-                        if (!mbar_wait_bounded(&acc_empty_bar[b], (buf / Cfg::kBuffers & 1) ^ 1, limit, abort_flag)) {
+                        if (!mbar_wait_bounded<CG == 2>(&acc_empty_bar[b], (buf / Cfg::kBuffers & 1) ^ 1, limit, abort_flag)) {
                             give_up(kStatusTimeoutMma);
                             ok = false;
                             break;
@@ -701,7 +701,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         acc = 0;
                     }
                     const int s = it % STAGES;
-                    if (!mbar_wait_bounded(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
+                    // (of loader warps and cleared tails: the peer's stores too, so acquired from the pair)
+                    if (!mbar_wait_bounded<CG == 2>(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
                         give_up(kStatusTimeoutMma);
                         ok = false;
                         break;
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 continue;
             }
             if (CG == 2) {
-                ok = __all_sync(~0u, mbar_wait_bounded(&peer_tail_bar[s], phase, limit, abort_flag));
+                ok = __all_sync(~0u, mbar_wait_bounded<true>(&peer_tail_bar[s], phase, limit, abort_flag));
                 if (!ok) {
                     if (lane == 0) give_up(kStatusTimeoutProducer);
                     break;
