@@ -658,142 +658,142 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 if (kAhead == 2 && ok && kb + 1 < t.kb) step_over(m[kAhead - 1], n[kAhead - 1], kb + 1);
             }
         }
-    } else if (!Cfg::TMA && warp > Cfg::kMmaWarp && warp < Cfg::kEpiWarp0) {
-        set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();  // the rest of the MMA's warpgroup
-    } else if (!Cfg::TMA && CG == 2 && warp == Cfg::kMmaWarp && !leader) {
-        set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();
-        // ------------------------------------------------------------ tells the leader of the peer's filled stages
-        if (lane == 0) {
-            int it = 0;
-            bool ok = true;
-            while (ok && work.next(t)) {
-                for (int kb = 0; kb < t.kb; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    if (!mbar_wait_bounded(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
-                        give_up(kStatusTimeoutProducer);
-                        ok = false;
-                        break;
+    } else if (warp < Cfg::kEpiWarp0) {
+        // By all warps of the MMA's warpgroup, the idle ones too: a warpgroup changes its share with one instruction.
+        if (!Cfg::TMA) set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();
+        if (!Cfg::TMA && CG == 2 && warp == Cfg::kMmaWarp && !leader) {
+            // ------------------------------------------------------------ tells the leader of the peer's filled stages
+            if (lane == 0) {
+                int it = 0;
+                bool ok = true;
+                while (ok && work.next(t)) {
+                    for (int kb = 0; kb < t.kb; ++kb, ++it) {
+                        const int s = it % STAGES;
+                        if (!mbar_wait_bounded(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
+                            give_up(kStatusTimeoutProducer);
+                            ok = false;
+                            break;
+                        }
+                        mbar_arrive_cluster(leader_bar(&full_bar[s]));
                     }
-                    mbar_arrive_cluster(leader_bar(&full_bar[s]));
                 }
             }
-        }
-    } else if (warp == Cfg::kMmaWarp) {
-        // ------------------------------------------------------------ MMA issuer (leader)
-        if (!Cfg::TMA) set_max_registers<Cfg::kMmaRegs, Cfg::kLaunchRegs>();
-        if (lane == 0 && leader) {
-            int it = 0, buf = 0;
-            bool ok = true;
-            while (ok && work.next(t)) {
-                const uint32_t idesc =
-                    umma_idesc_f16(Cfg::BM, t.cols, Cfg::M_MN, Cfg::N_MN, PLANES > 1 ? 1 : p.bf16);
-                uint32_t d_tmem = 0, acc = 0;
-                for (int kb = 0; kb < t.kb; ++kb, ++it) {
-                    if (kb % Cfg::kSumStages == 0) {
-                        const int b = buf % Cfg::kBuffers;
-                        if (!mbar_wait_bounded<CG == 2>(&acc_empty_bar[b], (buf / Cfg::kBuffers & 1) ^ 1, limit, abort_flag)) {
+        } else if (warp == Cfg::kMmaWarp) {
+            // ------------------------------------------------------------ MMA issuer (leader)
+            if (lane == 0 && leader) {
+                int it = 0, buf = 0;
+                bool ok = true;
+                while (ok && work.next(t)) {
+                    const uint32_t idesc =
+                        umma_idesc_f16(Cfg::BM, t.cols, Cfg::M_MN, Cfg::N_MN, PLANES > 1 ? 1 : p.bf16);
+                    uint32_t d_tmem = 0, acc = 0;
+                    for (int kb = 0; kb < t.kb; ++kb, ++it) {
+                        if (kb % Cfg::kSumStages == 0) {
+                            const int b = buf % Cfg::kBuffers;
+                            if (!mbar_wait_bounded<CG == 2>(&acc_empty_bar[b], (buf / Cfg::kBuffers & 1) ^ 1, limit, abort_flag)) {
+                                give_up(kStatusTimeoutMma);
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            d_tmem = tmem_base + b * NT;
+                            acc = 0;
+                        }
+                        const int s = it % STAGES;
+                        // (of loader warps and cleared tails: the peer's stores too, so acquired from the pair)
+                        if (!mbar_wait_bounded<CG == 2>(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
                             give_up(kStatusTimeoutMma);
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        d_tmem = tmem_base + b * NT;
-                        acc = 0;
-                    }
-                    const int s = it % STAGES;
-                    // (of loader warps and cleared tails: the peer's stores too, so acquired from the pair)
-                    if (!mbar_wait_bounded<CG == 2>(&full_bar[s], (it / STAGES) & 1, limit, abort_flag)) {
-                        give_up(kStatusTimeoutMma);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const int slabs = Cfg::KS == 1 ? 1 : min(Cfg::KS, t.slabs - kb * Cfg::KS);
-                    for (int j = 0; j < slabs; ++j) {
-                        // 16-deep steps of this slab that the contraction still has
-                        const int steps = min(kGroupedDepth / 16, t.steps - (kb * Cfg::KS + j) * (kGroupedDepth / 16));
-                        const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage + j * Cfg::kSlab);
-                        const uint64_t m_desc = umma_smem_desc(m_addr, Cfg::M_MN ? 8192 : 16, 1024, kLayoutSwizzle128B);
-                        const uint64_t n_desc =
-                            umma_smem_desc(m_addr + Cfg::kMBytes, Cfg::N_MN ? 8192 : 16, 1024, kLayoutSwizzle128B);
-                        const uint32_t m_lo = static_cast<uint32_t>(m_desc), m_hi = static_cast<uint32_t>(m_desc >> 32);
-                        const uint32_t n_lo = static_cast<uint32_t>(n_desc), n_hi = static_cast<uint32_t>(n_desc >> 32);
-                        auto mma = [&](int mp, int np, int ks) {  // descriptors count 16-byte units
-                            umma_f16<CG>(d_tmem, m_lo + (mp * Cfg::kMPlane + ks * (Cfg::M_MN ? 2048 : 32)) / 16, m_hi,
-                                         n_lo + (np * Cfg::kNPlane + ks * (Cfg::N_MN ? 2048 : 32)) / 16, n_hi, idesc, acc);
-                            acc = 1;
-                        };
-                        // The small products of all steps first: every addition truncates relative to what the
-                        // accumulator holds, so only the last four cut at the sum's own size.
-                        constexpr int kTerms = PLANES == 3 ? 6 : PLANES == 2 ? 3 : 1;
-                        constexpr int kMTerm[6] = {2, 0, 1, 1, 0, 0}, kNTerm[6] = {0, 2, 1, 0, 1, 0};
-                        if (steps == kGroupedDepth / 16) {
-#pragma unroll
-                            for (int i = 6 - kTerms; i < 6; ++i)
-#pragma unroll
-                                for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
-                        } else {
-#pragma unroll
-                            for (int i = 6 - kTerms; i < 6; ++i)
-                                for (int ks = 0; ks < steps; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                        const int slabs = Cfg::KS == 1 ? 1 : min(Cfg::KS, t.slabs - kb * Cfg::KS);
+                        for (int j = 0; j < slabs; ++j) {
+                            // 16-deep steps of this slab that the contraction still has
+                            const int steps = min(kGroupedDepth / 16, t.steps - (kb * Cfg::KS + j) * (kGroupedDepth / 16));
+                            const uint32_t m_addr = smem_u32(smem + s * Cfg::kStage + j * Cfg::kSlab);
+                            const uint64_t m_desc = umma_smem_desc(m_addr, Cfg::M_MN ? 8192 : 16, 1024, kLayoutSwizzle128B);
+                            const uint64_t n_desc =
+                                umma_smem_desc(m_addr + Cfg::kMBytes, Cfg::N_MN ? 8192 : 16, 1024, kLayoutSwizzle128B);
+                            const uint32_t m_lo = static_cast<uint32_t>(m_desc), m_hi = static_cast<uint32_t>(m_desc >> 32);
+                            const uint32_t n_lo = static_cast<uint32_t>(n_desc), n_hi = static_cast<uint32_t>(n_desc >> 32);
+                            auto mma = [&](int mp, int np, int ks) {  // descriptors count 16-byte units
+                                umma_f16<CG>(d_tmem, m_lo + (mp * Cfg::kMPlane + ks * (Cfg::M_MN ? 2048 : 32)) / 16, m_hi,
+                                             n_lo + (np * Cfg::kNPlane + ks * (Cfg::N_MN ? 2048 : 32)) / 16, n_hi, idesc, acc);
+                                acc = 1;
+                            };
+                            // The small products of all steps first: every addition truncates relative to what the
+                            // accumulator holds, so only the last four cut at the sum's own size.
+                            constexpr int kTerms = PLANES == 3 ? 6 : PLANES == 2 ? 3 : 1;
+                            constexpr int kMTerm[6] = {2, 0, 1, 1, 0, 0}, kNTerm[6] = {0, 2, 1, 0, 1, 0};
+                            if (steps == kGroupedDepth / 16) {
+    #pragma unroll
+                                for (int i = 6 - kTerms; i < 6; ++i)
+    #pragma unroll
+                                    for (int ks = 0; ks < kGroupedDepth / 16; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                            } else {
+    #pragma unroll
+                                for (int i = 6 - kTerms; i < 6; ++i)
+                                    for (int ks = 0; ks < steps; ++ks) mma(kMTerm[i], kNTerm[i], ks);
+                            }
+                        }
+                        if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
+                        else umma_commit(&empty_bar[s]);
+                        if (kb % Cfg::kSumStages == Cfg::kSumStages - 1 || kb == t.kb - 1) {
+                            if (CG == 2) umma_commit_pair(&acc_full_bar[buf % Cfg::kBuffers], 0x3);
+                            else umma_commit(&acc_full_bar[buf % Cfg::kBuffers]);
+                            ++buf;
                         }
                     }
-                    if (CG == 2) umma_commit_pair(&empty_bar[s], 0x3);
-                    else umma_commit(&empty_bar[s]);
-                    if (kb % Cfg::kSumStages == Cfg::kSumStages - 1 || kb == t.kb - 1) {
-                        if (CG == 2) umma_commit_pair(&acc_full_bar[buf % Cfg::kBuffers], 0x3);
-                        else umma_commit(&acc_full_bar[buf % Cfg::kBuffers]);
-                        ++buf;
-                    }
                 }
+                if (CG == 2) umma_commit_pair(drain_bar, 0x1);
+                else umma_commit(drain_bar);
+                if (!mbar_wait_drain(drain_bar, 0, limit)) report_status(kStatusTimeoutDrain, nullptr);
             }
-            if (CG == 2) umma_commit_pair(drain_bar, 0x1);
-            else umma_commit(drain_bar);
-            if (!mbar_wait_drain(drain_bar, 0, limit)) report_status(kStatusTimeoutDrain, nullptr);
-        }
-    } else if (Cfg::TMA && Cfg::RIGHT && warp == Cfg::kFixWarp) {
-        // ------------------------------------------------------------ clears the rows behind a group
-        // The last MMA step of a contraction over a group's rows may hold rows of the next group (or NaN of a
-        // buffer's spare rows): both operands' become 0 before the MMA may read them.
-        int it = 0;
-        uint32_t phases = 0;  // parities of each stage's tail barriers
-        bool ok = true;
-        while (ok && work.next(t)) {
-            const int rows = t.t1 - t.t0, valid = rows % kGroupedDepth, end = (valid + 15) / 16 * 16;
-            it += t.kb;
-            if (rows % 16 == 0) continue;
-            const int s = (it - 1) % STAGES;
-            const uint32_t phase = (phases >> s) & 1;
-            ok = mbar_wait_bounded(&tail_bar[s], phase, limit, abort_flag);
-            ok = __all_sync(~0u, ok);
-            if (!ok) {
-                if (lane == 0) give_up(kStatusTimeoutProducer);
-                break;
-            }
-            phases ^= 1u << s;
-            const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage + (t.slabs - 1) % Cfg::KS * Cfg::kSlab);
-            const int boxes = t.cols / CG / 64;
-            for (int b = 0; b < 2 + boxes; ++b) {
-                const uint32_t box = m_tile + (b < 2 ? b * 8192 : Cfg::kMBytes + (b - 2) * 8192);
-                for (int at = valid * 128 + lane * 16; at < end * 128; at += 512) store_shared16(box + at, 0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            // One arrival completes the stage: the leader's, after the peer's tail is cleared too.
-            if (CG == 2 && !leader) {
-                if (lane == 0) mbar_arrive_cluster(leader_bar(&peer_tail_bar[s]));
-                continue;
-            }
-            if (CG == 2) {
-                ok = __all_sync(~0u, mbar_wait_bounded<true>(&peer_tail_bar[s], phase, limit, abort_flag));
+        } else if (Cfg::TMA && Cfg::RIGHT && warp == Cfg::kFixWarp) {
+            // ------------------------------------------------------------ clears the rows behind a group
+            // The last MMA step of a contraction over a group's rows may hold rows of the next group (or NaN of a
+            // buffer's spare rows): both operands' become 0 before the MMA may read them.
+            int it = 0;
+            uint32_t phases = 0;  // parities of each stage's tail barriers
+            bool ok = true;
+            while (ok && work.next(t)) {
+                const int rows = t.t1 - t.t0, valid = rows % kGroupedDepth, end = (valid + 15) / 16 * 16;
+                it += t.kb;
+                if (rows % 16 == 0) continue;
+                const int s = (it - 1) % STAGES;
+                const uint32_t phase = (phases >> s) & 1;
+                ok = mbar_wait_bounded(&tail_bar[s], phase, limit, abort_flag);
+                ok = __all_sync(~0u, ok);
                 if (!ok) {
                     if (lane == 0) give_up(kStatusTimeoutProducer);
                     break;
                 }
+                phases ^= 1u << s;
+                const uint32_t m_tile = smem_u32(smem + s * Cfg::kStage + (t.slabs - 1) % Cfg::KS * Cfg::kSlab);
+                const int boxes = t.cols / CG / 64;
+                for (int b = 0; b < 2 + boxes; ++b) {
+                    const uint32_t box = m_tile + (b < 2 ? b * 8192 : Cfg::kMBytes + (b - 2) * 8192);
+                    for (int at = valid * 128 + lane * 16; at < end * 128; at += 512) store_shared16(box + at, 0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                // One arrival completes the stage: the leader's, after the peer's tail is cleared too.
+                if (CG == 2 && !leader) {
+                    if (lane == 0) mbar_arrive_cluster(leader_bar(&peer_tail_bar[s]));
+                    continue;
+                }
+                if (CG == 2) {
+                    ok = __all_sync(~0u, mbar_wait_bounded<true>(&peer_tail_bar[s], phase, limit, abort_flag));
+                    if (!ok) {
+                        if (lane == 0) give_up(kStatusTimeoutProducer);
+                        break;
+                    }
+                }
+                if (lane == 0) mbar_arrive(&full_bar[s]);
             }
-            if (lane == 0) mbar_arrive(&full_bar[s]);
         }
-    } else if (warp >= Cfg::kEpiWarp0) {
+    } else {
         // ------------------------------------------------------------ epilogue
         if (!Cfg::TMA) set_max_registers<Cfg::kEpiRegs, Cfg::kLaunchRegs>();
         const int quarter = warp & 3;                    // TMEM lanes of this warp
