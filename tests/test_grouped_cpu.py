@@ -96,3 +96,13 @@ def test_abi_rejects_outputs_over_the_offsets():
         for offsets, needle in ((C, "alias"), (C + 4, "alias"), (C - 4, "alias"), (C - 4096 + 2, "aligned")):
             assert entry(0, None, ctypes.byref(_desc()), offsets, A, B, C) == _lib.MFB_EINVAL
             assert needle in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(k=0, lda=1), dict(groups=0), dict(rows=0)])
+def test_abi_rejects_misaligned_outputs_of_calls_that_read_nothing(kw):
+    """Such calls still write zeros (rows of no group, empty sums)."""
+    lib = mf.lib()
+    entry = lib.mfb_grouped_gemm_bwd_right if "rows" in kw else lib.mfb_grouped_gemm
+    for c, types in ((C + 2, {}), (C + 1, dict(dtype=2, out_dtype=2)), (C + 2, dict(dtype=1))):
+        st = entry(0, None, ctypes.byref(_desc(**kw, **types)), O, A, B, c)
+        assert st == _lib.MFB_EINVAL and "aligned" in _lib.last_error()
