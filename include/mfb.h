@@ -363,7 +363,7 @@ typedef struct mfb_int4_matrix {
     unsigned char* packed;  /* 16-byte aligned */
     void* scales;           /* scale_dtype */
     unsigned char* zeros;   /* 0..15 each, or NULL */
-    int experts;            /* matrices in the stack (>= 1) */
+    int experts;            /* matrices in the stack (0: none, every row of mfb_gemv_int4 is then of no matrix) */
     int n, k;
     int group;              /* 32, 64 or 128 */
     int scale_dtype;        /* mfb_dtype_t */

@@ -744,7 +744,7 @@ mfb_status_t gemv_int4_launch(const Int4Params& p, int device, cudaStream_t stre
         const auto kernel = &gemv_int4_kernel<T, TS, GROUP, RT, HALVES>;
         const int chunks = (p.k + 128 * HALVES - 1) / (128 * HALVES);
         CUtensorMap map{};
-        if (p.k > 0) MFB_TRY(encode_codes(&map, p.packed, p.rows, p.row_bytes, HALVES));
+        if (p.k > 0 && p.rows > 0) MFB_TRY(encode_codes(&map, p.packed, p.rows, p.row_bytes, HALVES));
         static std::atomic<unsigned long long> raised{0};  // devices whose shared-memory limit is raised
         const unsigned long long bit = 1ull << (device & 63);
         if (!(raised.load(std::memory_order_acquire) & bit)) {

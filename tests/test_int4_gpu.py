@@ -311,3 +311,16 @@ def test_empty_calls():
     assert y.shape == (3, 8) and not y.any()
     q = mf.quantize_int4(torch.empty(0, 40, device="cuda"), 32)
     assert mf.dequantize_int4(q).shape == (0, 40)
+
+
+def test_empty_stack_gives_zero_rows():
+    for dtype in (F32, F16):
+        q = mf.quantize_int4(torch.empty(0, 24, 64, dtype=dtype, device="cuda"), 32)
+        x = _normal((3, 64), dtype, 1)
+        y = mf.gemv_int4(q, x, experts=torch.full((3,), -1, dtype=torch.int32, device="cuda"))
+        mf.sync()
+        assert q.shape == (0, 24, 64) and y.shape == (3, 24) and not y.any()
+        y = mf.gemv_int4(q, x, experts=torch.tensor([-1, 0, 5], dtype=torch.int32, device="cuda"))
+        with pytest.raises(mf.InvalidArgumentError):
+            mf.sync()
+        assert not y.any() and mf.dequantize_int4(q).shape == (0, 24, 64)
