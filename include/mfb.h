@@ -107,7 +107,8 @@ MFB_API const char* mfb_version(void);
 /* Reads and clears the device status word that bounded waits report into.
  * *bits receives the raw word (0 = nothing reported since the last read). Synchronizes
  * the device first. Returns MFB_ETIMEOUT when a wait gave up, MFB_EINVAL when kernels only
- * found group offsets or expert ids out of range. */
+ * found group offsets or expert ids out of range; only this call and mfb_sync report those
+ * (mfb_cuda_sync and the calls that wait for work of their own leave them to the next of these). */
 MFB_API mfb_status_t mfb_device_status(int device, uint32_t* bits);
 /* Bound, in nanoseconds of device time, for every device-side wait of later launches
  * (default 4e9 = 4 s). Process-wide. */

@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             v = max(v, floor);
             if (i <= p.groups) {
                 offset[i] = v;
-                if (v != raw && worker == 0 && leader) atomicOr(&g_status, kStatusBadIndex);
+                if (v != raw && worker == 0 && leader) report_bad_index();
             }
             int prev = __shfl_up_sync(~0u, v, 1);
             if (lane == 0) prev = floor;

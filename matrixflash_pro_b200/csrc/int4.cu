@@ -403,7 +403,7 @@ __device__ __forceinline__ void gemv_segments(const Int4Params& p, const int* id
         const int r = lane + 32 * h;
         id[h] = r < rows ? ids[r] : -1;
         if (id[h] >= p.experts) {
-            if (blockIdx.x == 0) atomicOr(&g_status, kStatusBadIndex);
+            if (blockIdx.x == 0) report_bad_index();
             id[h] = -1;
         }
     }

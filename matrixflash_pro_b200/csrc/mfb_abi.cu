@@ -161,11 +161,14 @@ mfb_status_t validate_desc(const mfb_gemm_desc* d, const float* a, const float* 
     return MFB_OK;
 }
 
-mfb_status_t read_and_clear_status(uint32_t* bits) {
-    uint32_t v = 0;
-    MFB_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_status, sizeof(v)), "status read");
-    const uint32_t zero = 0;
-    MFB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)), "status clear");
+mfb_status_t read_and_clear_status(uint32_t* bits, bool indices) {
+    uint32_t words[2] = {0, 0};
+    const size_t bytes = (indices ? 2 : 1) * sizeof(uint32_t);
+    MFB_CUDA_TRY(cudaMemcpyFromSymbol(words, g_status, bytes), "status read");
+    const uint32_t v = words[kStatusWaits] | words[kStatusIndices];
+    const uint32_t zero[2] = {0, 0};
+    // (nothing to clear: a bit that a kernel of another stream sets meanwhile stays)
+    if (v) MFB_CUDA_TRY(cudaMemcpyToSymbol(g_status, zero, bytes), "status clear");
     if (bits) *bits = v;
     if (v == kStatusBadIndex)
         return fail(MFB_EINVAL, "a kernel found group offsets or an expert id out of range");
@@ -271,15 +274,19 @@ MFB_API mfb_status_t mfb_device_status(int device, uint32_t* bits) {
     DeviceGuard guard;
     MFB_TRY(select_device(device));
     MFB_CUDA_TRY(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
-    return read_and_clear_status(bits);
+    return read_and_clear_status(bits, true);
+}
+
+static mfb_status_t sync_stream(int device, cudaStream_t stream, bool indices) {
+    DeviceGuard guard;
+    MFB_TRY(select_device(device));
+    MFB_CUDA_TRY(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
+    MFB_CUDA_TRY(cudaGetLastError(), "pending CUDA error");
+    return read_and_clear_status(nullptr, indices);
 }
 
 MFB_API mfb_status_t mfb_sync(int device, mfb_stream_t stream) {
-    DeviceGuard guard;
-    MFB_TRY(select_device(device));
-    MFB_CUDA_TRY(cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream)), "cudaStreamSynchronize");
-    MFB_CUDA_TRY(cudaGetLastError(), "pending CUDA error");
-    return read_and_clear_status(nullptr);
+    return sync_stream(device, reinterpret_cast<cudaStream_t>(stream), true);
 }
 
 MFB_API mfb_status_t mfb_sgemm(int device, mfb_stream_t stream_h, const mfb_gemm_desc* desc, const float* a,
@@ -672,7 +679,7 @@ MFB_API mfb_status_t mfb_cuda_sync(int device) {
     Slot* slot = nullptr;
     MFB_TRY(slot_for(device, &slot));
     std::lock_guard<std::mutex> lock(slot->mutex);
-    return mfb_sync(device, reinterpret_cast<mfb_stream_t>(slot->stream));
+    return sync_stream(device, slot->stream, false);
 }
 
 // ---------------------------------------------------------------- conv2d

@@ -9,9 +9,10 @@
 namespace mfb {
 
 // Status bits a kernel ORs into g_status when it gives up on a wait or finds an index in
-// device memory out of range. The host reads and clears the word (mfb_sync /
-// mfb_device_status) and maps kStatusBadIndex alone to MFB_EINVAL, any other bit to
-// MFB_ETIMEOUT.
+// device memory out of range. The host reads and clears a word and maps kStatusBadIndex
+// alone to MFB_EINVAL, any other bit to MFB_ETIMEOUT. kStatusBadIndex has a word of its own:
+// it is the caller's doing, so only mfb_sync and mfb_device_status read that one, while calls
+// that wait for their own kernels ask for waits alone.
 enum : uint32_t {
     kStatusTimeoutProducer = 1u << 0,   // TMA producer waited too long for a free stage
     kStatusTimeoutMma = 1u << 1,        // MMA issuer waited too long for a filled stage
@@ -24,7 +25,8 @@ enum : uint32_t {
 
 // Defined here: libmfb.so is one translation unit (csrc/libmfb.cu), so every kernel
 // names the same word without relocatable device code.
-__device__ uint32_t g_status = 0;
+enum : int { kStatusWaits = 0, kStatusIndices = 1 };
+__device__ uint32_t g_status[2] = {0, 0};
 
 __device__ __forceinline__ uint64_t globaltimer_ns() {
     uint64_t t;
@@ -123,9 +125,11 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ void report_status(uint32_t bits, volatile int* abort) {
-    atomicOr(&g_status, bits);
+    atomicOr(&g_status[kStatusWaits], bits);
     if (abort) *abort = 1;
 }
+
+__device__ __forceinline__ void report_bad_index() { atomicOr(&g_status[kStatusIndices], kStatusBadIndex); }
 
 // ----------------------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor, tiled, no multicast)

@@ -176,7 +176,8 @@ mfb_status_t naive_launch(const mfb_gemm_desc& d, cudaStream_t stream, const flo
 
 // ---------------------------------------------------------------------- probes
 mfb_status_t probe_wait_launch(cudaStream_t stream, uint64_t limit_ns);
-mfb_status_t read_and_clear_status(uint32_t* bits);
+// `indices`: also the word of indices out of range, which only mfb_sync and mfb_device_status report.
+mfb_status_t read_and_clear_status(uint32_t* bits, bool indices = false);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

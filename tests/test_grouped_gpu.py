@@ -431,3 +431,21 @@ def test_weight_gradient_of_many_ragged_groups(dtype, groups, most, k, n):
     for _ in range(10):
         assert torch.equal(mf.grouped_matmul_backward_right(d, x, off), first)
     assert mf.device_status() == 0
+
+
+def test_bad_offsets_are_no_other_calls_error():
+    """Calls that wait for work of their own neither fail by them nor take the report away from sync()."""
+    from matrixflash_pro_b200.distributed import sgemm_multi
+    x, w = _normal((10, 16), F32, 1), _normal((1, 16, 24), F32, 2)
+    a = _normal((128, 128), F32, 3)
+    plan = mf.GemmPlan(128, 128, 128, mf.GemmOptions())
+    calls = [lambda: plan.tune(a, a, torch.empty_like(a)), lambda: mf.probe_tf32_mma_tflops(), lambda: mf.cuda_sync(0),
+             lambda: sgemm_multi([a], a, [torch.empty_like(a)])]
+    for call in calls:
+        mf.device_status()
+        mf.grouped_matmul(x, w, torch.tensor([0, 11], dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        call()
+        with pytest.raises(mf.InvalidArgumentError):
+            mf.sync()
+        mf.sync()
