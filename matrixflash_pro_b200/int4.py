@@ -32,9 +32,10 @@ GEMV_ROWS = 64
 
 
 class Int4Matrix:
-    """A checked set of 4-bit codes, scales and zero points (layout: module text). Keeps the tensors."""
+    """A checked set of 4-bit codes, scales and zero points (layout: module text). Keeps the tensors, whose contents may
+    change; which tensors they are may not, since the kernels get their addresses."""
 
-    __slots__ = ("packed", "scales", "zeros", "k", "group", "n", "experts", "device", "_desc", "_ref")
+    __slots__ = ("_packed", "_scales", "_zeros", "_k", "_group", "_n", "_experts", "_device", "_desc", "_ref")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, k: int, group: int):
         k = checked_dim(k)
@@ -62,19 +63,28 @@ class Int4Matrix:
                 raise InvalidArgumentError("the parts of a 4-bit matrix must be contiguous")
         if packed.data_ptr() % 16:
             raise InvalidArgumentError("packed codes must start on a 16-byte boundary")
-        self.packed, self.scales, self.zeros, self.k, self.group = packed, scales, zeros, k, int(group)
-        self.n = checked_dim(packed.shape[-2])
-        self.experts = checked_dim(packed.shape[0]) if packed.dim() == 3 else None
-        self.device = packed.device
+        self._packed, self._scales, self._zeros, self._k, self._group = packed, scales, zeros, k, int(group)
+        self._n = checked_dim(packed.shape[-2])
+        self._experts = checked_dim(packed.shape[0]) if packed.dim() == 3 else None
+        self._device = packed.device
         self._desc = _lib.Int4MatrixDesc(packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
-                                         1 if self.experts is None else self.experts, self.n, k, self.group,
+                                         1 if self._experts is None else self._experts, self._n, k, self._group,
                                          DTYPES[scales.dtype])
         self._ref = ctypes.byref(self._desc)
+
+    packed = property(lambda self: self._packed, doc="The codes, two a byte.")
+    scales = property(lambda self: self._scales, doc="A scale per row and group.")
+    zeros = property(lambda self: self._zeros, doc="A zero point per row and group, or None.")
+    k = property(lambda self: self._k, doc="Columns.")
+    group = property(lambda self: self._group, doc="Columns that share a scale.")
+    n = property(lambda self: self._n, doc="Rows (of one matrix of a stack).")
+    experts = property(lambda self: self._experts, doc="Matrices in the stack, or None for a single matrix.")
+    device = property(lambda self: self._device, doc="The tensors' device.")
 
     @property
     def shape(self):
         """The shape of the weights that the codes stand for."""
-        return torch.Size((*self.packed.shape[:-1], self.k))
+        return torch.Size((*self._packed.shape[:-1], self._k))
 
 
 def quantize_int4(weight: torch.Tensor, group: int = 128, symmetric: bool = False,
@@ -139,11 +149,11 @@ def gemv_int4(matrix: Int4Matrix, x: torch.Tensor, out: torch.Tensor | None = No
     """y[r] = W x[r] for up to 64 rows of x [t,k] (float32, float16 or bfloat16); out [t,n] has x's type. A stack
     needs `experts`, a contiguous int32 CUDA tensor [t]: row r uses matrix experts[r]; a negative id gives a zero
     row, one past the stack a zero row and InvalidArgumentError from the next sync()."""
-    dtype, device = x.dtype, matrix.device
+    dtype, device = x.dtype, matrix._device
     code = DTYPES.get(dtype)
     if code is None:
         raise InvalidArgumentError("gemv_int4 takes float32, float16 or bfloat16 rows")
-    if x.dim() != 2 or x.shape[1] != matrix.k:
+    if x.dim() != 2 or x.shape[1] != matrix._k:
         raise ShapeMismatchError("GEMV operand shape mismatch")
     if x.device != device:
         raise InvalidArgumentError("x must be on the matrix's device")
@@ -151,7 +161,7 @@ def gemv_int4(matrix: Int4Matrix, x: torch.Tensor, out: torch.Tensor | None = No
     if rows > GEMV_ROWS:
         raise InvalidArgumentError(f"gemv_int4 serves up to {GEMV_ROWS} rows (dequantize_int4 and a product serve more)")
     ldx, unit = x.stride()
-    if unit != 1 and matrix.k > 1 and rows:
+    if unit != 1 and matrix._k > 1 and rows:
         raise InvalidArgumentError("x must have unit column stride")
     ids = 0
     if experts is not None:
@@ -162,9 +172,9 @@ def gemv_int4(matrix: Int4Matrix, x: torch.Tensor, out: torch.Tensor | None = No
         if experts.device != device:
             raise InvalidArgumentError("experts must be on the matrix's device")
         ids = experts.data_ptr()
-    elif matrix.experts is not None:
+    elif matrix._experts is not None:
         raise InvalidArgumentError("a stack of matrices needs an expert per row")
-    n = matrix.n
+    n = matrix._n
     if out is None:
         out, ldy = _new(x, (rows, n), dtype, stream), n
     else:

@@ -104,3 +104,11 @@ def test_abi_rejects_outputs_over_the_matrix(at):
     assert "alias" in _lib.last_error()
     assert lib.mfb_gemv_int4(0, None, m, 1, X, 64, 0, Y + 66, Y, 4) == _lib.MFB_EINVAL
     assert "aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("name", ["packed", "scales", "zeros", "k", "group", "n", "experts", "device", "shape"])
+def test_the_parts_of_a_matrix_cannot_be_exchanged(name):
+    """The kernels get addresses that were taken when the matrix was made."""
+    matrix = object.__new__(mf.Int4Matrix)
+    with pytest.raises(AttributeError):
+        setattr(matrix, name, None)
