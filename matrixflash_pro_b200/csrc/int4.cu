@@ -323,6 +323,9 @@ struct GemvX8 {
                 for (int t = 1; t < TERMS; ++t) {
                     lo -= __uint_as_float(v[t - 1][i] << 16);
                     hi -= __uint_as_float(v[t - 1][i] & 0xffff0000u);
+                    // An infinity is its own first term, and the others are 0 (inf - inf is NaN). A NaN stays one.
+                    if (t == 1 && __uint_as_float(w[2 * i] & 0x7fffffffu) == __int_as_float(0x7f800000)) lo = 0.0f;
+                    if (t == 1 && __uint_as_float(w[2 * i + 1] & 0x7fffffffu) == __int_as_float(0x7f800000)) hi = 0.0f;
                     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[t][i]) : "f"(hi), "f"(lo));
                 }
             }

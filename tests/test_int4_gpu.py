@@ -324,3 +324,18 @@ def test_empty_stack_gives_zero_rows():
         with pytest.raises(mf.InvalidArgumentError):
             mf.sync()
         assert not y.any() and mf.dequantize_int4(q).shape == (0, 24, 64)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+def test_infinite_rows(dtype):
+    """An infinite value gives what the products of the formula give: an infinity of the weight's sign, or NaN where the
+    weight is 0 or infinities of both signs meet. The largest finite value is no infinity."""
+    m = _matrix(0, 70, 300, 64, True, F32, 3)
+    x = _normal((5, 300), dtype, 4)
+    x[0, 7], x[1, 299], x[2, 3], x[2, 130], x[3, 64] = float("inf"), float("-inf"), float("inf"), float("inf"), torch.finfo(dtype).max
+    y = mf.gemv_int4(m, x)
+    mf.sync()
+    ref = (x.double() @ _values(m).t())[:3]
+    assert (ref == float("inf")).any() and (ref == float("-inf")).any() and ref.isnan().any()
+    assert torch.equal(y[:3].double().nan_to_num(7.0, float("inf"), float("-inf")), ref.nan_to_num(7.0, float("inf"), float("-inf")))
+    assert not y[3:].isnan().any() and y[4].isfinite().all()
