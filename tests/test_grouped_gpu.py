@@ -449,3 +449,16 @@ def test_bad_offsets_are_no_other_calls_error():
         with pytest.raises(mf.InvalidArgumentError):
             mf.sync()
         mf.sync()
+
+
+@pytest.mark.parametrize("e", [-110, -118, -126, -136])
+def test_values_below_the_third_terms_range(e):
+    """Under 2^-110 a value's third BF16 term falls below that type's smallest number, 2^-133: each loses up to 2^-134
+    more than elsewhere."""
+    x = torch.ldexp(_normal((70, 200), F32, 1).double(), torch.tensor(e, device="cuda")).float()
+    w = _normal((1, 200, 96), F32, 2)
+    off = _offsets([70])
+    y, s = _reference(x, w, off)
+    got = mf.grouped_matmul(x, w, off)
+    mf.sync()
+    assert ((got.double() - y).abs() <= _bound(y, s, 200, F32) + 2.0 ** -134 * w[0].double().abs().sum(0)).all()

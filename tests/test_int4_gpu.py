@@ -339,3 +339,16 @@ def test_infinite_rows(dtype):
     assert (ref == float("inf")).any() and (ref == float("-inf")).any() and ref.isnan().any()
     assert torch.equal(y[:3].double().nan_to_num(7.0, float("inf"), float("-inf")), ref.nan_to_num(7.0, float("inf"), float("-inf")))
     assert not y[3:].isnan().any() and y[4].isfinite().all()
+
+
+@pytest.mark.parametrize("e", [-110, -118, -126, -136])
+def test_values_below_the_third_terms_range(e):
+    """Under 2^-110 a value's third BF16 term falls below that type's smallest number, 2^-133: each loses up to 2^-134
+    more than elsewhere."""
+    m = _matrix(0, 96, 200, 128, True, F32, 1)
+    x = torch.ldexp(_normal((8, 200), F32, 2).double(), torch.tensor(e, device="cuda")).float()
+    y = mf.gemv_int4(m, x)
+    mf.sync()
+    w = _values(m)
+    ref, s = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    assert ((y.double() - ref).abs() <= U * (200 / 8 + 32) * s + 2.0 ** -134 * w.abs().sum(1)).all()
