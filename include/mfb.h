@@ -343,9 +343,11 @@ typedef struct mfb_grouped_desc {
 } mfb_grouped_desc;
 
 /* C[t] = A[t] * op(B_e) for every row t of group e: A rows x k, B_e k x n (n x k with trans_b),
- * C rows x n. Products of the operands' own bits, sums in FP32, one rounding to out_dtype; FP32
- * operands as three BF16 terms each (strict) or two (MFB_PRECISION_TF32). The gradient by A is
- * the same call on the gradient rows with trans_b flipped. k == 0 gives 0. Takes no scratch. */
+ * C rows x n. Products of the operands' own bits, sums in FP32 (up to 512 of the contraction,
+ * strict FP32 64, added with truncation by the tensor cores, the rest with rounding), one rounding
+ * to out_dtype; FP32 operands as three BF16 terms each (strict; an infinity gives NaN, values below
+ * 2^-110 lose up to 2^-134) or two (MFB_PRECISION_TF32). The gradient by A is the same call on the
+ * gradient rows with trans_b flipped. k == 0 gives 0. Takes no scratch. */
 MFB_API mfb_status_t mfb_grouped_gemm(int device, mfb_stream_t stream, const mfb_grouped_desc* desc,
                                       const int* offsets, const void* a, const void* b, void* c);
 /* C_e = sum over rows t of group e of A[t]^T B[t] (k x n; A rows x k, B rows x n): the gradient by
@@ -372,17 +374,18 @@ typedef struct mfb_int4_matrix {
 
 /* Codes of w (element strides: row ldw, matrix stride_w; finite values). With zeros: over a group,
  * lo = min(0, w), hi = max(0, w), s = (hi - lo) / 15, z = rint(-lo / s); without: s = max|w| / 7.
- * s is rounded to scale_dtype (saturating; 0 becomes 1) before the codes, q = rint(w / s) + z
- * clamped to 0..15, ties to even, decided on the exact quotient. */
+ * s is rounded through FP32 to scale_dtype (saturating; 0 becomes 1) before the codes, q =
+ * rint(w / s) + z clamped to 0..15, ties to even, decided on the exact quotient. */
 MFB_API mfb_status_t mfb_quantize_int4(int device, mfb_stream_t stream, const void* w, int dtype, long long ldw,
                                        long long stride_w, const mfb_int4_matrix* out);
-/* out = (q - z) * s, rounded once to `dtype`. */
+/* out = (q - z) * s in FP32 (exact for 16-bit scales), rounded to `dtype`. */
 MFB_API mfb_status_t mfb_dequantize_int4(int device, mfb_stream_t stream, const mfb_int4_matrix* m, void* out,
                                          int dtype, long long ldo, long long stride_o);
 /* y[r] = W x[r] for rows r of x (rows x k, row stride ldx) and y (rows x n, row stride ldy), both of
  * `dtype`; the products take the codes exactly and sums are FP32. rows <= MFB_INT4_GEMV_ROWS. With
  * expert_ids (device memory, one int per row) row r uses matrix expert_ids[r] of the stack; a negative
- * id gives a zero row, one >= experts a zero row and MFB_EINVAL from the next mfb_sync. */
+ * id gives a zero row, one >= experts a zero row and MFB_EINVAL from the next mfb_sync. Infinite
+ * values give what the formula gives; FP32 values below 2^-110 lose up to 2^-134. */
 #define MFB_INT4_GEMV_ROWS 64
 MFB_API mfb_status_t mfb_gemv_int4(int device, mfb_stream_t stream, const mfb_int4_matrix* m, int rows, const void* x,
                                    long long ldx, int dtype, const int* expert_ids, void* y, long long ldy);

@@ -198,6 +198,10 @@ mfb_status_t launch_grouped(int device, const mfb_grouped_desc& d, cudaStream_t 
     // narrow / wide, by rows per group: 16 27.0 / 28.2, 48 28.3 / 29.9, 64 37.7 / 30.3, 128 55.7 / 32.3 (bf16);
     // 16 127 / 128, 48 128 / 130, 64 177 / 131 (FP32): a group of more than 64 rows reads its weights twice in narrow
     // tiles. Gradient by the matrices, 8 groups of 256 rows, n = 2048, by k: 64 7.0 / 9.0, 128 8.8 / 9.0, 256 12.7 / 9.8.
+    // The host knows the mean alone, and skewed groups want wide tiles at smaller means. 8 experts of 2048x4096, one of 340
+    // rows and seven of 6: 35.5 / 31.1 (bf16), 159 / 165 (FP32); 32 of 2048x1024, eight of 100 and the others of 2: 36.8 /
+    // 32.1, 161 / 119; 64 of 512x1024, four of 470 and the others of 2: 21.1 / 21.3, 75 / 83 (even groups of 31: 18.8 / 21.1,
+    // 65 / 70). So the rule loses up to a sixth (FP32: a third) on skewed groups, and would lose as much on even ones at 30.
     const bool wide = right ? d.k > 64 : d.rows / std::max(1, d.groups) > 48;
     const GroupedEntry e = size == 2 ? (tma ? entry_of<1, true>(right, m_mn, wide) : entry_of<1, false>(right, m_mn, wide))
                            : d.precision == MFB_PRECISION_FP32 ? entry_of<3, false>(right, m_mn, wide)

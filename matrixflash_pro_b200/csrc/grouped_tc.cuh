@@ -13,22 +13,25 @@
 // 16-bit operands whose rows TMA can address come by TMA, 64 of the contraction deep, 128-byte swizzle
 // (K-major tiles a box of rows, MN-major tiles boxes of 64 columns). All others (FP32, odd
 // strides) come by loader warps that read global memory into registers and write the same layout:
-// 16-bit values as they are, FP32 as PLANES BF16 terms x = h + m + l (h cut, m and l rounded; exact with
-// three). Products hh, hm, mh, mm, hl, lh are kept (six MMAs per step, 1/6 of the BF16 rate); what is left
-// out is below 2^-21 of |a b|. Two terms (TF32 precision) keep hh, hm, mh.
+// 16-bit values as they are, FP32 as PLANES BF16 terms x = h + m + l (h cut, m and l rounded). Three are exact down
+// to 2^-110; below, l falls under BF16's smallest number and up to 2^-134 of x is lost. An infinity has no terms
+// (inf - inf) and gives NaN. Products hh, hm, mh, mm, hl, lh are kept (six MMAs per step, 1/6 of the BF16 rate); what
+// is left out is below 2^-21 of |a b|. Two terms (TF32 precision) keep hh, hm, mh.
 //
 // The tensor core adds with truncation, so the accumulator restarts every 64 of the contraction (strict FP32) or 512
 // (all others) and the epilogue warps add the chunks, rounding to nearest: the error does not grow with the
 // contraction. (FP32 every 128 instead would save 5% of the time and take the error at k = 4096 from 1.9e-7 to 6e-7.)
-// 16-bit operands, k = 4096, 8 experts of 1024 rows, by the chunk: 256 662 us, error of the sums 2.4e-7 (all products
-// positive 3.8e-7); 512 589 us, 4.8e-7 (9e-7); 1024 573 us, 1e-6 (2.2e-6); never restarted 552 us, 4.4e-6 (1.4e-5,
-// and 8e-5 at k = 16384). 512 is the longest that stays below 1e-6. What it costs is the hand-over: the next chunk's MMAs
+// 16-bit operands, k = 4096, 8 experts of 1024 rows, graph replay, by the chunk: 256 662 us, error of the sums 2.4e-7
+// (all products positive 3.8e-7); 512 589 us, 4.8e-7 (9e-7); 1024 573 us, 1e-6 (2.2e-6); never restarted 552 us, 4.4e-6
+// (1.4e-5, and 8e-5 at k = 16384). 512 is the longest that keeps sums of both signs below 1e-6 for both types (BF16 as
+// given, FP16 6.5e-7; 2.8e-6 where all products are positive). What it costs is the hand-over: the next chunk's MMAs
 // wait for a buffer whose reader needs 3600 cycles, signals across the pair included, and a chunk's MMAs take 4096.
 //
-// Bounds, and what it reaches on a B200: 8192 rows over 8 experts, 4096x11008 bf16, 539 us, 1370 TFLOP/s, the
-// tensor core under the power limit (cuBLAS sustains 1387); 32 rows over 32 experts, 2048x1024 bf16, 25.8 us,
-// 3.4 TB/s of weights (160 tiles for 148 SMs); FP32, 3000 rows over 16 experts, 1024x2048,
-// 113 to 142 us by GPU, about 105 TFLOP/s of the 279 that six MMAs allow, the work on the terms and a last wave.
+// Bounds, and what it reaches on a B200: 8192 rows over 8 experts, 4096x11008 bf16, single calls 570 us, 1296 TFLOP/s,
+// the hand-over of chunks and a last wave (1376 tiles for 74 pairs); call after call 687 us, 1075 TFLOP/s, at 1.3 GHz
+// under the power limit (cuBLAS sustains 1387). 32 rows over 32 experts, 2048x1024 bf16, 26.4 us by graph replay, 3.3
+// TB/s (160 tiles for 148 SMs). FP32, 3000 rows over 16 experts, 1024x2048, 114 to 171 us by GPU, about 100 TFLOP/s
+// of the 279 that six MMAs allow, the work on the terms and a last wave (tensor pipe 38% busy, issue slots 44%).
 #pragma once
 
 #include "mfb_device.cuh"

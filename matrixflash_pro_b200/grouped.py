@@ -13,7 +13,11 @@ With transpose_right the weights (and their gradient) are stored [e,n,k].
 Operands are float32 (strict, as GemmPrecision.fp32; tf32 permits fewer terms), float16 or
 bfloat16 CUDA tensors of one type with unit stride in the last dimension; rows and matrices may be
 padded or shared (strides are taken from the tensors, 0 between matrices reuses one weight). Sums
-are FP32, rounded once; an infinite float32 operand gives NaN (it has no terms to split into).
+are FP32: the tensor cores add up to 512 of the contraction (strict float32: 64) with truncation,
+those chunks are added with rounding, and the result is rounded once to the output's type. So the error
+of the sums does not grow with their length: 5e-7 normwise for bfloat16, 7e-7 for float16 (9e-7 and 3e-6
+where all products are positive), 3e-7 for strict float32, measured up to 16384 products. An infinite
+float32 operand gives NaN (it has no terms to split into); those below 2^-110 lose up to 2^-134.
 `out` may be given, of the operands' type or float32, and may overlap nothing that the call reads.
 
 offsets is a contiguous int32 CUDA tensor of e + 1 entries that the kernels read: the host never

@@ -90,8 +90,8 @@ class Int4Matrix:
 def quantize_int4(weight: torch.Tensor, group: int = 128, symmetric: bool = False,
                   scale_dtype: torch.dtype | None = None, stream=None) -> Int4Matrix:
     """Codes of `weight` ([n,k] or [e,n,k], float32, float16 or bfloat16, finite). symmetric: s = max|w| / 7 and
-    no zero points; else s and z span the group's range, widened to hold 0. Scales take scale_dtype (default:
-    the weight's); codes are the nearest ones, ties to even."""
+    no zero points; else s and z span the group's range, widened to hold 0. Scales are rounded through FP32 to
+    scale_dtype (default: the weight's); codes are the nearest ones, ties to even."""
     if weight.dtype not in DTYPES:
         raise InvalidArgumentError("quantize_int4 takes float32, float16 or bfloat16 weights")
     if weight.dim() not in (2, 3):
@@ -119,7 +119,8 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, symmetric: bool = Fals
 
 def dequantize_int4(matrix: Int4Matrix, dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                     stream=None) -> torch.Tensor:
-    """The weights (q - z) * s of `matrix`, rounded once to `dtype` (default: the scales')."""
+    """The weights (q - z) * s of `matrix` in FP32 (exact for 16-bit scales), rounded to `dtype` (default: the
+    scales')."""
     if out is None:
         dtype = matrix.scales.dtype if dtype is None else dtype
         if dtype not in DTYPES:
@@ -148,7 +149,8 @@ def gemv_int4(matrix: Int4Matrix, x: torch.Tensor, out: torch.Tensor | None = No
               experts: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """y[r] = W x[r] for up to 64 rows of x [t,k] (float32, float16 or bfloat16); out [t,n] has x's type. A stack
     needs `experts`, a contiguous int32 CUDA tensor [t]: row r uses matrix experts[r]; a negative id gives a zero
-    row, one past the stack a zero row and InvalidArgumentError from the next sync()."""
+    row, one past the stack a zero row and InvalidArgumentError from the next sync(). Sums are FP32. An infinite x
+    gives the infinities (or NaN, at a weight of 0) of the formula; float32 values of x below 2^-110 lose up to 2^-134."""
     dtype, device = x.dtype, matrix._device
     code = DTYPES.get(dtype)
     if code is None:
